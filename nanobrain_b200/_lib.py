@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI declared in ``include/nb_attn.h``.
+"""ctypes binding of the C ABI declared in ``include/nb_attn.h`` and ``include/nb_block.h``.
 
 The structures below mirror the header field by field. There is deliberately no fallback: if
 the shared library is missing or cannot be loaded, importing an entry point raises.
@@ -29,6 +29,16 @@ EXPORTED_SYMBOLS = (
     "nb_attn_schedule_capacity",
     "nb_attn_schedule_build",
     "nb_attn_schedule_host",
+)
+# Every symbol include/nb_block.h declares.
+BLOCK_SYMBOLS = (
+    "nb_qk_norm_rope_fwd",
+    "nb_qk_norm_rope_bwd",
+    "nb_qk_norm_rope_bwd_workspace_bytes",
+    "nb_gated_mlp_fwd",
+    "nb_gated_mlp_bwd",
+    "nb_gated_mlp_bwd_workspace_bytes",
+    "nb_gated_mlp_checkpoint_bytes",
 )
 BUILTIN_SCRATCH_ROWS = 65536
 BUILTIN_SCRATCH_ITEMS = 16384
@@ -101,6 +111,74 @@ class BwdArgs(C.Structure):
     ]
 
 
+class QkSide(C.Structure):
+    _fields_ = [
+        ("x", Tensor),
+        ("y", Tensor),
+        ("dy", Tensor),
+        ("weight", C.c_void_p),
+        ("d_weight", C.c_void_p),
+        ("positions", C.c_void_p),
+        ("position_stride_batch", C.c_int64),
+        ("position_stride_token", C.c_int64),
+        ("heads", C.c_int32),
+        ("tokens", C.c_int32),
+    ]
+
+
+class QkNormRopeArgs(C.Structure):
+    _fields_ = [
+        ("q", QkSide),
+        ("k", QkSide),
+        ("batch", C.c_int32),
+        ("axes", C.c_int32),
+        ("position_type", C.c_int32),
+        ("interleaved", C.c_int32),
+        ("freqs", C.c_void_p),
+        ("eps", C.c_float),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class Matrix(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("stride", C.c_int64)]
+
+
+class GatedMlpShape(C.Structure):
+    _fields_ = [
+        ("tokens", C.c_int64),
+        ("dim", C.c_int32),
+        ("hidden", C.c_int32),
+        ("activation", C.c_int32),
+        ("checkpoint", C.c_int32),
+    ]
+
+
+class GatedMlpFwdArgs(C.Structure):
+    _fields_ = [
+        ("shape", GatedMlpShape),
+        *[(name, Matrix) for name in ("x", "w_gate", "w_up", "w_down", "y")],
+        *[(name, C.c_void_p) for name in ("b_gate", "b_up", "b_down")],
+        ("h", Matrix),
+        ("checkpoint", C.c_void_p),
+        ("status", C.c_void_p),
+    ]
+
+
+class GatedMlpBwdArgs(C.Structure):
+    _fields_ = [
+        ("shape", GatedMlpShape),
+        *[(name, Matrix) for name in ("x", "w_gate", "w_up", "w_down", "dy", "h")],
+        ("checkpoint", C.c_void_p),
+        *[(name, Matrix) for name in ("dx", "d_w_gate", "d_w_up", "d_w_down")],
+        *[(name, C.c_void_p) for name in ("d_b_gate", "d_b_up", "d_b_down")],
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+        ("status", C.c_void_p),
+    ]
+
+
 _lib = None
 
 
@@ -145,6 +223,16 @@ def load() -> C.CDLL:
     lib.nb_attn_bwd_builtin_scratch.argtypes = [C.POINTER(BwdArgs), C.c_void_p]
     lib.nb_attn_selftest_mma.restype = C.c_int
     lib.nb_attn_selftest_mma.argtypes = [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
+    for name, args in (("nb_qk_norm_rope_fwd", QkNormRopeArgs), ("nb_qk_norm_rope_bwd", QkNormRopeArgs),
+                       ("nb_gated_mlp_fwd", GatedMlpFwdArgs), ("nb_gated_mlp_bwd", GatedMlpBwdArgs)):
+        getattr(lib, name).restype = C.c_int
+        getattr(lib, name).argtypes = [C.POINTER(args), C.c_void_p]
+    lib.nb_qk_norm_rope_bwd_workspace_bytes.restype = C.c_size_t
+    lib.nb_qk_norm_rope_bwd_workspace_bytes.argtypes = []
+    lib.nb_gated_mlp_bwd_workspace_bytes.restype = C.c_size_t
+    lib.nb_gated_mlp_bwd_workspace_bytes.argtypes = [C.POINTER(GatedMlpBwdArgs)]
+    lib.nb_gated_mlp_checkpoint_bytes.restype = C.c_size_t
+    lib.nb_gated_mlp_checkpoint_bytes.argtypes = [C.POINTER(GatedMlpShape)]
     got = lib.nb_attn_abi_version()
     if got != ABI_VERSION:
         raise RuntimeError(f"libnb_attn.so has ABI version {got}, this package expects {ABI_VERSION}")

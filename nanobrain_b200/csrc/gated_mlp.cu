@@ -1,0 +1,621 @@
+// The gated feed-forward block of include/nb_block.h: host side, the form for few tokens and the kernels that finish
+// what gemm_kernel.cuh leaves in parts.
+//
+// Forward: one launch for a, b and h (kGemmGate), one for y. Backward: one for da, db (kGemmDact), one for dx and the
+// three weight gradients together (kGemmPlain), and where needed one that adds split products up and two for the biases.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "../../include/nb_block.h"
+#include "gemm_kernel.cuh"
+#include "host.h"
+
+namespace {
+
+using namespace nb;
+using bf16 = __nv_bfloat16;
+
+// ---- few tokens, forward only ----------------------------------------------------------------
+// Bound by reading the weights once: a warp takes a feature (a row of Wg and of Wu, or of Wd), its lanes 16 bytes at a
+// time, and applies it to all tokens. On tensor cores the 4096 weight rows of ViT-B's block would occupy 32 of 148 SMs.
+constexpr int kFewTokens = 8, kFewWarps = 4;
+
+__device__ __forceinline__ float dot8(const uint4& w, const uint4& x, float acc) {
+  const uint32_t a[4] = {w.x, w.y, w.z, w.w}, b[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    acc = fmaf(__uint_as_float(a[i] << 16), __uint_as_float(b[i] << 16), acc);
+    acc = fmaf(__uint_as_float(a[i] & 0xFFFF0000u), __uint_as_float(b[i] & 0xFFFF0000u), acc);
+  }
+  return acc;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+
+struct FewParams {
+  const bf16 *x, *w0, *w1, *bias0, *bias1;
+  bf16* out;
+  int64_t xs, w0s, w1s, outs;
+  int32_t tokens, in, out_n;
+};
+
+template <int kAct, int kTokens>
+__global__ void __launch_bounds__(kFewWarps * 32) few_gate_kernel(const __grid_constant__ FewParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, f = blockIdx.x * kFewWarps + (threadIdx.x >> 5);
+  if (f >= p.out_n) return;
+  const bf16 *wg = p.w0 + f * p.w0s, *wu = p.w1 + f * p.w1s;
+  float a[kTokens], b[kTokens];
+#pragma unroll
+  for (int t = 0; t < kTokens; ++t) a[t] = b[t] = 0.f;
+#pragma unroll 4
+  for (int c = lane * 8; c < p.in; c += 256) {
+    const uint4 g = *reinterpret_cast<const uint4*>(wg + c), u = *reinterpret_cast<const uint4*>(wu + c);
+#pragma unroll
+    for (int t = 0; t < kTokens; ++t) {
+      if (t >= p.tokens) break;
+      const uint4 x = *reinterpret_cast<const uint4*>(p.x + t * p.xs + c);
+      a[t] = dot8(g, x, a[t]), b[t] = dot8(u, x, b[t]);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < kTokens; ++t) a[t] = warp_sum(a[t]), b[t] = warp_sum(b[t]);
+  if (lane != 0) return;
+  const float bg = p.bias0 != nullptr ? __bfloat162float(p.bias0[f]) : 0.f;
+  const float bu = p.bias1 != nullptr ? __bfloat162float(p.bias1[f]) : 0.f;
+#pragma unroll
+  for (int t = 0; t < kTokens; ++t)
+    if (t < p.tokens) p.out[t * p.outs + f] = __float2bfloat16(gate_of<kAct>(a[t] + bg) * (b[t] + bu));
+}
+
+constexpr int kFewAhead = 8;  // pieces of a lane's weights requested before the kernel in front is done
+template <int kTokens>
+__global__ void __launch_bounds__(kFewWarps * 32) few_down_kernel(const __grid_constant__ FewParams p) {
+  const int lane = threadIdx.x & 31, d = blockIdx.x * kFewWarps + (threadIdx.x >> 5);
+  const bf16* w = p.w0 + int64_t(min(d, p.out_n - 1)) * p.w0s;
+  // The gate kernel, which comes right in front, does not write weights.
+  uint4 ahead[kFewAhead];
+#pragma unroll
+  for (int i = 0; i < kFewAhead; ++i) {
+    const int c = lane * 8 + i * 256;
+    ahead[i] = c < p.in ? *reinterpret_cast<const uint4*>(w + c) : make_uint4(0, 0, 0, 0);
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+  float y[kTokens];
+#pragma unroll
+  for (int t = 0; t < kTokens; ++t) y[t] = 0.f;
+#pragma unroll
+  for (int i = 0; i < kFewAhead; ++i) {
+    const int c = lane * 8 + i * 256;
+    if (c >= p.in) break;
+#pragma unroll
+    for (int t = 0; t < kTokens; ++t) {
+      if (t >= p.tokens) break;
+      y[t] = dot8(ahead[i], *reinterpret_cast<const uint4*>(p.x + t * p.xs + c), y[t]);
+    }
+  }
+#pragma unroll 4
+  for (int c = lane * 8 + kFewAhead * 256; c < p.in; c += 256) {
+    const uint4 g = *reinterpret_cast<const uint4*>(w + c);
+#pragma unroll
+    for (int t = 0; t < kTokens; ++t) {
+      if (t >= p.tokens) break;
+      y[t] = dot8(g, *reinterpret_cast<const uint4*>(p.x + t * p.xs + c), y[t]);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < kTokens; ++t) y[t] = warp_sum(y[t]);
+  if (lane != 0 || d >= p.out_n) return;
+  const float bias = p.bias0 != nullptr ? __bfloat162float(p.bias0[d]) : 0.f;
+#pragma unroll
+  for (int t = 0; t < kTokens; ++t)
+    if (t < p.tokens) p.out[t * p.outs + d] = __float2bfloat16(y[t] + bias);
+}
+
+// ---- what is left in parts ---------------------------------------------------------------------
+// The sum of a split product's parts, in their order. A thread takes a row's eight columns.
+struct SplitItem {
+  const float4* partial;
+  bf16* out;
+  int64_t stride;
+  int32_t rows, n, row_tiles, col_tiles, cols, splits;
+  int64_t pieces;  // of 8 columns x 1 row, over whole tiles
+};
+struct SplitParams {
+  SplitItem item[3];
+  int32_t n_items;
+};
+__global__ void __launch_bounds__(256) split_sum_kernel(const __grid_constant__ SplitParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  int i = 0;
+  while (i < p.n_items && at >= p.item[i].pieces) at -= p.item[i++].pieces;
+  if (i == p.n_items) return;
+  const SplitItem& s = p.item[i];
+  const int row = int(at % kGemmRows);
+  const int64_t block = at / kGemmRows;  // (tile, eight columns)
+  const int per = s.cols / 8;
+  const int tile = int(block / per), oct = int(block % per);
+  const int64_t whole = int64_t(s.row_tiles) * s.col_tiles * (s.cols / 4) * kGemmRows;
+  const float4* src = s.partial + (int64_t(tile) * (s.cols / 4) + 2 * oct) * kGemmRows + row;
+  float4 a = src[0], b = src[kGemmRows];
+  for (int k = 1; k < s.splits; ++k) {
+    const float4 x = src[k * whole], y = src[k * whole + kGemmRows];
+    a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
+    b.x += y.x, b.y += y.y, b.z += y.z, b.w += y.w;
+  }
+  const int64_t r = int64_t(tile / s.col_tiles) * kGemmRows + row;
+  const int c = (tile % s.col_tiles) * s.cols + 8 * oct;
+  if (r < s.rows && c < s.n)
+    *reinterpret_cast<uint4*>(s.out + r * s.stride + c) =
+        make_uint4(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w), pack_bf16(b.x, b.y), pack_bf16(b.z, b.w));
+}
+
+// Sums of a matrix' columns over chunks of kSumRows rows: a block takes 64 columns.
+constexpr int kSumRows = 512;
+__global__ void __launch_bounds__(256) col_partial_kernel(const bf16* m, int64_t stride, int64_t rows, int n, float* out) {
+  __shared__ float part[32][65];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int oct = threadIdx.x & 7, lane = threadIdx.x >> 3, c = blockIdx.x * 64 + oct * 8;
+  float s[8] = {};
+  const int64_t first = int64_t(blockIdx.y) * kSumRows, last = first + kSumRows < rows ? first + kSumRows : rows;
+  if (c < n) {
+#pragma unroll 4
+    for (int64_t r = first + lane; r < last; r += 32) {
+      const uint4 v = *reinterpret_cast<const uint4*>(m + r * stride + c);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[2 * i] += __uint_as_float(w[i] << 16), s[2 * i + 1] += __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) part[lane][oct * 8 + i] = s[i];
+  __syncthreads();
+  if (threadIdx.x < 64 && blockIdx.x * 64 + threadIdx.x < n) {
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v += part[i][threadIdx.x];
+    out[int64_t(blockIdx.y) * n + blockIdx.x * 64 + threadIdx.x] = v;
+  }
+}
+
+struct ColItem {
+  const float* partial;  // [rows][stride]
+  bf16* out;
+  int64_t stride;
+  int32_t rows, n, blocks;
+};
+struct ColParams {
+  ColItem item[3];
+  int32_t n_items;
+};
+__global__ void __launch_bounds__(1024) col_sum_kernel(const __grid_constant__ ColParams p) {
+  __shared__ float part[32][33];
+  pdl_wait();
+  pdl_launch_dependents();
+  int b = blockIdx.x, i = 0;
+  while (b >= p.item[i].blocks) b -= p.item[i++].blocks;
+  const ColItem& s = p.item[i];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = b * 32 + lane;
+  float v = 0.f;
+  if (c < s.n) {
+#pragma unroll 8
+    for (int r = warp; r < s.rows; r += 32) v += s.partial[r * s.stride + c];
+  }
+  part[warp][lane] = v;
+  __syncthreads();
+  if (warp == 0 && c < s.n) {
+    v = 0.f;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) v += part[k][lane];
+    s.out[c] = __float2bfloat16(v);
+  }
+}
+
+// ---- host --------------------------------------------------------------------------------------
+template <typename... KArgs, typename... Args>
+int launch(void (*kernel)(KArgs...), dim3 grid, unsigned threads, size_t smem, void* stream, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? NB_ATTN_OK : NB_ATTN_ERR_LAUNCH;
+}
+
+// A GEMM kernel needs its shared memory allowed once per device.
+constexpr int kMaxDevices = 64;
+template <int kKind, int kAct, int kBits, int kProblems>
+int launch_gemm(const GemmParams<kProblems>& g, int sms, void* stream) {
+  static std::mutex mutex;
+  static bool ready[kMaxDevices];
+  auto* kernel = gemm_kernel<kKind, kAct, kBits, kProblems>;
+  constexpr int kSmem = GemmSmem<kKind>::kBytes;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return NB_ATTN_ERR_DEVICE;
+  {
+    std::lock_guard<std::mutex> lock(mutex);
+    if (!ready[dev]) {
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
+        return NB_ATTN_ERR_LAUNCH;
+      ready[dev] = true;
+    }
+  }
+  const int units = g.deal.n_long + g.deal.n_short;
+  return launch(kernel, dim3(unsigned(std::min(units, sms))), kGemmThreads, kSmem, stream, g);
+}
+
+int div_up(int64_t a, int64_t b) { return int((a + b - 1) / b); }
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+// Columns of a tile, a multiple of `unit`, by the clocks that a CTA's share of the tiles takes: a 64-deep step's MMAs
+// take two clocks a column, but not less than its operands' 128-byte reads from shared memory; a tile also costs its
+// epilogue's start.
+int tile_cols(int row_tiles, int n, int steps, int sms, int unit) {
+  int best = kGemmMaxCols;
+  double least = 0;
+  for (int cols = kGemmMaxCols; cols >= unit; cols -= unit) {
+    const int64_t tiles = int64_t(row_tiles) * div_up(n, cols);
+    const double step = std::max(2.0 * cols, 128.0 + cols);
+    const double cost = double((tiles + sms - 1) / sms) * (steps * step + 800.0);
+    if (cols == kGemmMaxCols || cost < 0.97 * least) best = cols, least = cost;
+  }
+  return best;
+}
+
+int check_matrix(const nb_matrix& m, int64_t cols) {
+  if (m.ptr == nullptr) return NB_ATTN_ERR_NULL;
+  if ((reinterpret_cast<uintptr_t>(m.ptr) & 15u) != 0 || m.stride % 8 != 0 || m.stride < cols || m.stride >> 36) return NB_ATTN_ERR_ALIGN;
+  return NB_ATTN_OK;
+}
+int check_bias(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0 ? NB_ATTN_ERR_ALIGN : NB_ATTN_OK; }
+
+constexpr int kMaxWidth = 1 << 20;
+int check_shape(const nb_gated_mlp_shape& s) {
+  if (s.tokens <= 0 || s.dim <= 0 || s.hidden <= 0 || s.dim % 8 || s.hidden % 8) return NB_ATTN_ERR_SHAPE;
+  if (s.dim > kMaxWidth || s.hidden > kMaxWidth || s.tokens > INT32_MAX - kGemmRows) return NB_ATTN_ERR_SHAPE;
+  // Tiles are counted in 32 bits, of 64 columns at the least.
+  const int64_t rows = div_up(s.tokens, kGemmRows);
+  if (rows * div_up(std::max(s.dim, s.hidden), 64) > INT32_MAX / 4) return NB_ATTN_ERR_SHAPE;
+  if (s.activation != NB_ACT_SILU && s.activation != NB_ACT_GELU) return NB_ATTN_ERR_SHAPE;
+  if (s.checkpoint < NB_CHECKPOINT_NONE || s.checkpoint > NB_CHECKPOINT_8BIT) return NB_ATTN_ERR_SHAPE;
+  return NB_ATTN_OK;
+}
+
+size_t code_bytes(const nb_gated_mlp_shape& s) {
+  const size_t blocks = size_t(div_up(s.tokens, kGemmRows)) * div_up(s.hidden, kGroup);
+  return blocks * kGemmRows * kGroup * 2 * (s.checkpoint == NB_CHECKPOINT_8BIT ? 1 : 2);
+}
+
+// Boxes of an operand whose inner index runs along memory: 64 deep x rows; of the others: 64 x 64.
+int map_k_major(CUtensorMap* m, const nb_matrix& t, int64_t rows, int64_t cols, int box_rows) {
+  return host_matrix_map(m, t.ptr, rows, cols, t.stride, box_rows, 64);
+}
+int map_mn_major(CUtensorMap* m, const nb_matrix& t, int64_t rows, int64_t cols) {
+  return host_matrix_map(m, t.ptr, rows, cols, t.stride, 64, 64);
+}
+
+#define NB_TRY(expr)                 \
+  do {                               \
+    if (const int rc_ = (expr)) return rc_; \
+  } while (0)
+
+template <int kAct, int kTokens>
+int launch_few(const nb_gated_mlp_fwd_args& a, void* stream) {
+  const nb_gated_mlp_shape& s = a.shape;
+  FewParams p{};
+  p.x = static_cast<const bf16*>(a.x.ptr), p.xs = a.x.stride;
+  p.w0 = static_cast<const bf16*>(a.w_gate.ptr), p.w0s = a.w_gate.stride;
+  p.w1 = static_cast<const bf16*>(a.w_up.ptr), p.w1s = a.w_up.stride;
+  p.bias0 = static_cast<const bf16*>(a.b_gate), p.bias1 = static_cast<const bf16*>(a.b_up);
+  p.out = static_cast<bf16*>(a.h.ptr), p.outs = a.h.stride;
+  p.tokens = int(s.tokens), p.in = s.dim, p.out_n = s.hidden;
+  NB_TRY(launch(few_gate_kernel<kAct, kTokens>, dim3(div_up(s.hidden, kFewWarps)), kFewWarps * 32, 0, stream, p));
+  FewParams d{};
+  d.x = p.out, d.xs = p.outs;
+  d.w0 = static_cast<const bf16*>(a.w_down.ptr), d.w0s = a.w_down.stride;
+  d.bias0 = static_cast<const bf16*>(a.b_down);
+  d.out = static_cast<bf16*>(a.y.ptr), d.outs = a.y.stride;
+  d.tokens = int(s.tokens), d.in = s.hidden, d.out_n = s.dim;
+  return launch(few_down_kernel<kTokens>, dim3(div_up(s.dim, kFewWarps)), kFewWarps * 32, 0, stream, d);
+}
+template <int kAct>
+int launch_few(const nb_gated_mlp_fwd_args& a, void* stream) {
+  if (a.shape.tokens == 1) return launch_few<kAct, 1>(a, stream);
+  if (a.shape.tokens == 2) return launch_few<kAct, 2>(a, stream);
+  return a.shape.tokens <= 4 ? launch_few<kAct, 4>(a, stream) : launch_few<kAct, kFewTokens>(a, stream);
+}
+
+template <int kKind, int kAct>
+int launch_bits(const GemmParams<1>& g, int checkpoint, int sms, void* stream) {
+  switch (checkpoint) {
+    case NB_CHECKPOINT_16BIT: return launch_gemm<kKind, kAct, 16, 1>(g, sms, stream);
+    case NB_CHECKPOINT_8BIT: return launch_gemm<kKind, kAct, 8, 1>(g, sms, stream);
+  }
+  if constexpr (kKind == kGemmGate) return launch_gemm<kKind, kAct, 0, 1>(g, sms, stream);
+  return NB_ATTN_ERR_SHAPE;
+}
+template <int kKind>
+int launch_act(const GemmParams<1>& g, const nb_gated_mlp_shape& s, int sms, void* stream) {
+  return s.activation == NB_ACT_SILU ? launch_bits<kKind, kActSilu>(g, s.checkpoint, sms, stream)
+                                     : launch_bits<kKind, kActGelu>(g, s.checkpoint, sms, stream);
+}
+
+void set_tiles(GemmProblem* p, int64_t rows, int n, int cols_of_tile, int per_tile, int steps0, int steps) {
+  p->n = n;
+  p->row_tiles = div_up(rows, kGemmRows);
+  p->cols = cols_of_tile;
+  p->col_tiles = div_up(n, per_tile);
+  p->steps0 = steps0, p->steps = steps;
+  p->splits = 1, p->split_steps = steps;
+}
+
+// Where the backward's scratch lies in the workspace, and how the weight gradients are cut.
+struct BwdPlan {
+  size_t da, db, h, col_sums, dy_sums, parts[3], bytes;
+  int cols[3], splits[3], split_steps[3];  // of dWg, dWu, dWd
+  int dx_cols;
+};
+
+BwdPlan plan_bwd(const nb_gated_mlp_bwd_args& a, int sms) {
+  const nb_gated_mlp_shape& s = a.shape;
+  BwdPlan p{};
+  size_t at = 0;
+  const auto take = [&at](size_t n) {
+    const size_t here = at;
+    at += align256(n);
+    return here;
+  };
+  const size_t hidden_bytes = size_t(s.tokens) * s.hidden * 2;
+  p.da = take(hidden_bytes), p.db = take(hidden_bytes);
+  p.h = take(s.checkpoint == NB_CHECKPOINT_8BIT ? hidden_bytes : 0);
+  const int row_tiles = div_up(s.tokens, kGemmRows);
+  p.col_sums = take(a.d_b_gate != nullptr || a.d_b_up != nullptr ? size_t(row_tiles) * 4 * 2 * s.hidden * 4 : 0);
+  p.dy_sums = take(a.d_b_down != nullptr ? size_t(div_up(s.tokens, kSumRows)) * s.dim * 4 : 0);
+  // A weight gradient's unit runs over all tokens. Where that is more than a CTA's even share of the launch's work, it is
+  // cut into parts of about half a share, which are added up behind (fp32, in a fixed order).
+  const int dx_steps = 2 * div_up(s.hidden, kGemmDepth), dw_steps = div_up(s.tokens, kGemmDepth);
+  const bool wanted[3] = {a.d_w_gate.ptr != nullptr, a.d_w_up.ptr != nullptr, a.d_w_down.ptr != nullptr};
+  p.dx_cols = tile_cols(row_tiles, s.dim, dx_steps, sms, 64);
+  double total = a.dx.ptr != nullptr ? double(row_tiles) * div_up(s.dim, p.dx_cols) * p.dx_cols * dx_steps : 0.0;
+  for (int i = 0; i < 3; ++i) {
+    const int rows = i < 2 ? s.hidden : s.dim, n = i < 2 ? s.dim : s.hidden;
+    p.cols[i] = (div_up(n, div_up(n, kGemmMaxCols)) + 63) / 64 * 64;
+    if (wanted[i]) total += double(div_up(rows, kGemmRows)) * div_up(n, p.cols[i]) * p.cols[i] * dw_steps;
+  }
+  for (int i = 0; i < 3; ++i) {
+    const int rows = i < 2 ? s.hidden : s.dim, n = i < 2 ? s.dim : s.hidden;
+    const double share = total / sms / p.cols[i];  // in steps
+    int splits = 1;
+    if (dw_steps > 0.8 * share) splits = std::min(div_up(dw_steps, 8), int(dw_steps / std::max(0.5 * share, 8.0)) + 1);
+    splits = std::max(1, std::min(splits, 32));
+    p.split_steps[i] = div_up(dw_steps, splits);
+    p.splits[i] = div_up(dw_steps, p.split_steps[i]);
+    const size_t tiles = size_t(div_up(rows, kGemmRows)) * div_up(n, p.cols[i]);
+    p.parts[i] = take(wanted[i] && p.splits[i] > 1 ? tiles * p.cols[i] * kGemmRows * 4 * p.splits[i] : 0);
+  }
+  p.bytes = std::max<size_t>(at, 256);
+  return p;
+}
+
+}  // namespace
+
+extern "C" size_t nb_gated_mlp_checkpoint_bytes(const nb_gated_mlp_shape* shape) {
+  if (shape == nullptr || check_shape(*shape) != NB_ATTN_OK || shape->checkpoint == NB_CHECKPOINT_NONE) return 0;
+  const size_t scales = size_t(div_up(shape->tokens, kGemmRows)) * div_up(shape->hidden, kGroup) * kGemmRows * 4;
+  return code_bytes(*shape) + scales;
+}
+
+extern "C" int nb_gated_mlp_fwd(const nb_gated_mlp_fwd_args* args, void* stream) {
+  if (args == nullptr) return NB_ATTN_ERR_NULL;
+  const nb_gated_mlp_shape& s = args->shape;
+  NB_TRY(check_shape(s));
+  NB_TRY(check_matrix(args->x, s.dim));
+  NB_TRY(check_matrix(args->w_gate, s.dim));
+  NB_TRY(check_matrix(args->w_up, s.dim));
+  NB_TRY(check_matrix(args->w_down, s.hidden));
+  NB_TRY(check_matrix(args->y, s.dim));
+  NB_TRY(check_matrix(args->h, s.hidden));
+  for (const void* b : {args->b_gate, args->b_up, args->b_down}) NB_TRY(check_bias(b));
+  if (s.checkpoint != NB_CHECKPOINT_NONE) {
+    if (args->checkpoint == nullptr) return NB_ATTN_ERR_NULL;
+    if ((reinterpret_cast<uintptr_t>(args->checkpoint) & 255u) != 0) return NB_ATTN_ERR_ALIGN;
+  }
+  int sms = 0;
+  NB_TRY(host_prepare(&sms));
+  if (s.checkpoint == NB_CHECKPOINT_NONE && s.tokens <= kFewTokens)
+    return s.activation == NB_ACT_SILU ? launch_few<kActSilu>(*args, stream) : launch_few<kActGelu>(*args, stream);
+
+  const int row_tiles = div_up(s.tokens, kGemmRows), steps = div_up(s.dim, kGemmDepth);
+  GemmParams<1> g{};
+  GemmProblem& p = g.p[0];
+  const int cols = tile_cols(row_tiles, 2 * s.hidden, steps, sms, 128);
+  set_tiles(&p, s.tokens, s.hidden, cols, cols / 2, steps, steps);
+  NB_TRY(map_k_major(&p.a[0], args->x, s.tokens, s.dim, kGemmRows));
+  NB_TRY(map_k_major(&p.b[0], args->w_gate, s.hidden, s.dim, cols / 2));
+  NB_TRY(map_k_major(&p.b[1], args->w_up, s.hidden, s.dim, cols / 2));
+  NB_TRY(host_matrix_map(&p.c, args->h.ptr, s.tokens, s.hidden, args->h.stride, kGemmRows, 64));
+  p.bias = static_cast<const bf16*>(args->b_gate);
+  g.bias_up = static_cast<const bf16*>(args->b_up);
+  g.codes = args->checkpoint;
+  g.scales = reinterpret_cast<uint32_t*>(static_cast<char*>(args->checkpoint) + code_bytes(s));
+  g.groups = div_up(s.hidden, kGroup), g.hidden = s.hidden;
+  g.deal.n_short = p.row_tiles * p.col_tiles;
+  g.status = args->status;
+
+  GemmParams<1> d{};
+  GemmProblem& q = d.p[0];
+  const int down_steps = div_up(s.hidden, kGemmDepth), down_cols = tile_cols(row_tiles, s.dim, down_steps, sms, 64);
+  set_tiles(&q, s.tokens, s.dim, down_cols, down_cols, down_steps, down_steps);
+  NB_TRY(map_k_major(&q.a[0], args->h, s.tokens, s.hidden, kGemmRows));
+  NB_TRY(map_k_major(&q.b[0], args->w_down, s.dim, s.hidden, down_cols));
+  NB_TRY(host_matrix_map(&q.c, args->y.ptr, s.tokens, s.dim, args->y.stride, kGemmRows, 64));
+  q.bias = static_cast<const bf16*>(args->b_down);
+  d.deal.n_short = q.row_tiles * q.col_tiles;
+  d.status = args->status;
+  NB_TRY(launch_act<kGemmGate>(g, s, sms, stream));
+  return launch_gemm<kGemmPlain, 0, 0, 1>(d, sms, stream);
+}
+
+extern "C" size_t nb_gated_mlp_bwd_workspace_bytes(const nb_gated_mlp_bwd_args* args) {
+  int sms = 0;
+  if (args == nullptr || check_shape(args->shape) != NB_ATTN_OK || host_prepare(&sms) != NB_ATTN_OK) return 0;
+  return plan_bwd(*args, sms).bytes;
+}
+
+extern "C" int nb_gated_mlp_bwd(const nb_gated_mlp_bwd_args* args, void* stream) {
+  if (args == nullptr) return NB_ATTN_ERR_NULL;
+  const nb_gated_mlp_bwd_args& a = *args;
+  const nb_gated_mlp_shape& s = a.shape;
+  NB_TRY(check_shape(s));
+  if (s.checkpoint == NB_CHECKPOINT_NONE) return NB_ATTN_ERR_SHAPE;
+  NB_TRY(check_matrix(a.x, s.dim));
+  NB_TRY(check_matrix(a.w_gate, s.dim));
+  NB_TRY(check_matrix(a.w_up, s.dim));
+  NB_TRY(check_matrix(a.w_down, s.hidden));
+  NB_TRY(check_matrix(a.dy, s.dim));
+  if (s.checkpoint == NB_CHECKPOINT_16BIT) NB_TRY(check_matrix(a.h, s.hidden));
+  if (a.dx.ptr != nullptr) NB_TRY(check_matrix(a.dx, s.dim));
+  if (a.d_w_gate.ptr != nullptr) NB_TRY(check_matrix(a.d_w_gate, s.dim));
+  if (a.d_w_up.ptr != nullptr) NB_TRY(check_matrix(a.d_w_up, s.dim));
+  if (a.d_w_down.ptr != nullptr) NB_TRY(check_matrix(a.d_w_down, s.hidden));
+  if (a.d_b_down != nullptr && s.tokens > int64_t(65535) * kSumRows) return NB_ATTN_ERR_SHAPE;  // (the sums' grid)
+  if (a.checkpoint == nullptr) return NB_ATTN_ERR_NULL;
+  if ((reinterpret_cast<uintptr_t>(a.checkpoint) & 255u) != 0 || (reinterpret_cast<uintptr_t>(a.workspace) & 255u) != 0)
+    return NB_ATTN_ERR_ALIGN;
+  int sms = 0;
+  NB_TRY(host_prepare(&sms));
+  const BwdPlan plan = plan_bwd(a, sms);
+  if (a.workspace == nullptr || a.workspace_bytes < plan.bytes) return NB_ATTN_ERR_WORKSPACE;
+  char* ws = static_cast<char*>(a.workspace);
+  const nb_matrix da{ws + plan.da, s.hidden}, db{ws + plan.db, s.hidden};
+  const nb_matrix h = s.checkpoint == NB_CHECKPOINT_8BIT ? nb_matrix{ws + plan.h, s.hidden} : a.h;
+  const int row_tiles = div_up(s.tokens, kGemmRows);
+
+  // dh = dy Wd with the activation's backward behind it. (Needed for every gradient but those of Wd, in 16 bits, and bd.)
+  const bool hidden_grads = a.dx.ptr != nullptr || a.d_w_gate.ptr != nullptr || a.d_w_up.ptr != nullptr ||
+                            a.d_b_gate != nullptr || a.d_b_up != nullptr;
+  const bool dact = hidden_grads || (a.d_w_down.ptr != nullptr && s.checkpoint == NB_CHECKPOINT_8BIT);
+  GemmParams<1> act{};
+  if (dact) {
+    GemmParams<1>& g = act;
+    GemmProblem& p = g.p[0];
+    const int steps = div_up(s.dim, kGemmDepth), cols = tile_cols(row_tiles, s.hidden, steps, sms, 64);
+    set_tiles(&p, s.tokens, s.hidden, cols, cols, steps, steps);
+    p.b_mn = 1;
+    NB_TRY(map_k_major(&p.a[0], a.dy, s.tokens, s.dim, kGemmRows));
+    NB_TRY(map_mn_major(&p.b[0], a.w_down, s.dim, s.hidden));
+    NB_TRY(host_matrix_map(&p.c, da.ptr, s.tokens, s.hidden, da.stride, kGemmRows, kGroup));
+    NB_TRY(host_matrix_map(&g.db, db.ptr, s.tokens, s.hidden, db.stride, kGemmRows, kGroup));
+    if (s.checkpoint == NB_CHECKPOINT_8BIT)
+      NB_TRY(host_matrix_map(&g.h, h.ptr, s.tokens, s.hidden, h.stride, kGemmRows, kGroup));
+    g.codes = const_cast<void*>(a.checkpoint);
+    g.scales = reinterpret_cast<uint32_t*>(static_cast<char*>(g.codes) + code_bytes(s));
+    g.groups = div_up(s.hidden, kGroup), g.hidden = s.hidden;
+    if (a.d_b_gate != nullptr || a.d_b_up != nullptr) g.col_sums = reinterpret_cast<float*>(ws + plan.col_sums);
+    g.deal.n_short = p.row_tiles * p.col_tiles;
+    g.status = a.status;
+  }
+
+  // dx and the weight gradients.
+  GemmParams<4> g{};
+  g.status = a.status;
+  const int hidden_steps = div_up(s.hidden, kGemmDepth), dw_steps = div_up(s.tokens, kGemmDepth);
+  int n = 0, dw_units = 0, dx_units = 0;
+  const auto add_dx = [&]() -> int {
+    if (a.dx.ptr == nullptr) return NB_ATTN_OK;
+    GemmProblem& p = g.p[n++];
+    set_tiles(&p, s.tokens, s.dim, plan.dx_cols, plan.dx_cols, hidden_steps, 2 * hidden_steps);
+    p.b_mn = 1;
+    NB_TRY(map_k_major(&p.a[0], da, s.tokens, s.hidden, kGemmRows));
+    NB_TRY(map_k_major(&p.a[1], db, s.tokens, s.hidden, kGemmRows));
+    NB_TRY(map_mn_major(&p.b[0], a.w_gate, s.hidden, s.dim));
+    NB_TRY(map_mn_major(&p.b[1], a.w_up, s.hidden, s.dim));
+    dx_units = p.row_tiles * p.col_tiles;
+    return host_matrix_map(&p.c, a.dx.ptr, s.tokens, s.dim, a.dx.stride, kGemmRows, 64);
+  };
+  SplitParams sums{};
+  const auto add_dw = [&](int which, const nb_matrix& left, const nb_matrix& right, const nb_matrix& out) -> int {
+    if (out.ptr == nullptr) return NB_ATTN_OK;
+    GemmProblem& p = g.p[n++];
+    const int rows = which < 2 ? s.hidden : s.dim, cols = which < 2 ? s.dim : s.hidden;
+    set_tiles(&p, rows, cols, plan.cols[which], plan.cols[which], dw_steps, dw_steps);
+    p.a_mn = p.b_mn = 1;
+    p.splits = plan.splits[which], p.split_steps = plan.split_steps[which];
+    NB_TRY(map_mn_major(&p.a[0], left, s.tokens, rows));
+    NB_TRY(map_mn_major(&p.b[0], right, s.tokens, cols));
+    dw_units += p.row_tiles * p.col_tiles * p.splits;
+    if (p.splits > 1) {
+      p.partial = reinterpret_cast<float*>(ws + plan.parts[which]);
+      SplitItem& i = sums.item[sums.n_items++];
+      i.partial = reinterpret_cast<const float4*>(p.partial);
+      i.out = static_cast<bf16*>(out.ptr), i.stride = out.stride;
+      i.rows = rows, i.n = cols, i.row_tiles = p.row_tiles, i.col_tiles = p.col_tiles, i.cols = p.cols;
+      i.splits = p.splits;
+      i.pieces = int64_t(p.row_tiles) * p.col_tiles * (p.cols / 8) * kGemmRows;
+      return NB_ATTN_OK;
+    }
+    return host_matrix_map(&p.c, out.ptr, rows, cols, out.stride, kGemmRows, 64);
+  };
+  // The longer units first.
+  const bool dw_first = std::max({plan.split_steps[0], plan.split_steps[1], plan.split_steps[2]}) >= 2 * hidden_steps;
+  if (!dw_first) NB_TRY(add_dx());
+  NB_TRY(add_dw(0, da, a.x, a.d_w_gate));
+  NB_TRY(add_dw(1, db, a.x, a.d_w_up));
+  NB_TRY(add_dw(2, a.dy, h, a.d_w_down));
+  if (dw_first) NB_TRY(add_dx());
+  if (dact) NB_TRY(launch_act<kGemmDact>(act, s, sms, stream));
+  if (n > 0) {
+    const int n_long = dw_first ? dw_units : dx_units, n_short = dw_first ? dx_units : dw_units;
+    g.deal.n_long = n_long, g.deal.n_short = n_short;
+    const int grid = std::min(n_long + n_short, sms), rem = n_long % grid;
+    if (n_short > 0 && rem > 0) {
+      const int dw_len = plan.split_steps[0], dx_len = 2 * hidden_steps;
+      const int ratio = dw_first ? dw_len / dx_len : dx_len / std::max(1, dw_len);
+      g.deal.extra = std::min(ratio, n_short / (grid - rem));
+    }
+    NB_TRY((launch_gemm<kGemmPlain, 0, 0, 4>(g, sms, stream)));
+  }
+  if (sums.n_items > 0) {
+    int64_t pieces = 0;
+    for (int i = 0; i < sums.n_items; ++i) pieces += sums.item[i].pieces;
+    NB_TRY(launch(split_sum_kernel, dim3(unsigned((pieces + 255) / 256)), 256, 0, stream, sums));
+  }
+
+  // Biases.
+  ColParams cols{};
+  const auto add_col = [&](void* out, const float* partial, int64_t stride, int rows, int width) {
+    if (out == nullptr) return;
+    cols.item[cols.n_items++] = ColItem{partial, static_cast<bf16*>(out), stride, rows, width, div_up(width, 32)};
+  };
+  const float* sums_at = reinterpret_cast<const float*>(ws + plan.col_sums);
+  add_col(a.d_b_gate, sums_at, 2 * int64_t(s.hidden), row_tiles * 4, s.hidden);
+  add_col(a.d_b_up, sums_at + s.hidden, 2 * int64_t(s.hidden), row_tiles * 4, s.hidden);
+  if (a.d_b_down != nullptr) {
+    float* dy_sums = reinterpret_cast<float*>(ws + plan.dy_sums);
+    const int chunks = div_up(s.tokens, kSumRows);
+    NB_TRY(launch(col_partial_kernel, dim3(div_up(s.dim, 64), chunks), 256, 0, stream, static_cast<const bf16*>(a.dy.ptr),
+                  a.dy.stride, s.tokens, int(s.dim), dy_sums));
+    add_col(a.d_b_down, dy_sums, s.dim, chunks, s.dim);
+  }
+  if (cols.n_items > 0) {
+    int blocks = 0;
+    for (int i = 0; i < cols.n_items; ++i) blocks += cols.item[i].blocks;
+    NB_TRY(launch(col_sum_kernel, dim3(blocks), 1024, 0, stream, cols));
+  }
+  return NB_ATTN_OK;
+}

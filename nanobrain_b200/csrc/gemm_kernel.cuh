@@ -1,0 +1,515 @@
+// Matrix products of the gated feed-forward block on the tensor cores, with what surrounds them in their epilogues:
+//
+//   kGemmGate   a = x Wg^T, b = x Wu^T over one pass of x; h = act(a) b and the checkpoint of a and b leave
+//   kGemmDact   dh = dy Wd; with a and b from the checkpoint da = dh b act'(a) and db = dh act(a) leave (and h again)
+//   kGemmPlain  up to four products of one launch, e.g. dx = da Wg + db Wu, dWg = da^T x, dWu = db^T x, dWd = dy^T h
+//
+// One persistent CTA per SM: warp 0 drives TMA, one thread of warp 1 issues tcgen05.mma, warps 4-11 are two epilogue
+// warpgroups. A unit is an output tile of 128 rows x up to 256 columns over a range of 64-deep steps. A and B tiles
+// are 64 elements (128 bytes, swizzled) x rows whichever way the matrix lies in memory: where the inner index runs
+// along memory the tile is a K-major operand, otherwise an MN-major one, so no product needs a transposed copy.
+// Accumulators are two sets of 256 tensor-memory columns: the epilogue of a unit runs under the products of the next.
+//
+// 128 x 256 columns because both operands come from shared memory: a 16-deep MMA takes 128 clocks and reads 12 KB, 96
+// clocks of the shared-memory port; 128 x 128 would read 8 KB in 64.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "ptx.cuh"
+
+namespace nb {
+
+constexpr int kGemmRows = 128, kGemmDepth = 64, kGemmMaxCols = 256;
+constexpr int kGemmThreads = 384;
+constexpr int kGemmBytesA = kGemmRows * kGemmDepth * 2, kGemmBytesB = kGemmMaxCols * kGemmDepth * 2;
+constexpr int kGemmStageBytes = kGemmBytesA + kGemmBytesB;
+constexpr int kGroup = 32;  // features of a token that share a scale in the checkpoint
+
+enum GemmKind { kGemmGate = 0, kGemmDact = 1, kGemmPlain = 2 };
+
+// Shared memory: stages, then the epilogue's staging (a part per warpgroup), then barriers.
+template <int kKind>
+struct GemmSmem {
+  static constexpr int kStages = kKind == kGemmDact ? 3 : 4;
+  static constexpr int kStagingWg = kKind == kGemmDact ? 3 * 8192 : 16384;
+  static constexpr int kStaging = kStages * kGemmStageBytes;
+  static constexpr int kBars = kStaging + 2 * kStagingWg;
+  static constexpr int kBytes = kBars + 256 + 1024;  // (+ 1024: the base is aligned by hand)
+};
+
+struct GemmProblem {
+  CUtensorMap a[2], b[2], c;  // a, b: of the two ranges of steps (gate: b of Wg and Wu)
+  const __nv_bfloat16* bias;  // per column, or NULL
+  float* partial;             // [split][row tile][column tile][columns / 4][128 rows][4], where splits > 1
+  int32_t n;                  // columns of the output
+  int32_t row_tiles, col_tiles, cols;  // cols: of a tile
+  int32_t steps0, steps;      // 64-deep steps of the first range, of both
+  int32_t splits, split_steps;
+  int32_t a_mn, b_mn;         // the operand's inner index does not run along memory
+};
+
+// The units of a launch, dealt to the CTAs in a fixed manner: `n_long` units (the problems with more steps come first
+// in the list) in turns; the CTAs left with one long unit fewer then take `extra` short ones each, and the rest of
+// the short units goes round again.
+struct GemmDeal {
+  int32_t n_long, n_short, extra;
+  __device__ __forceinline__ int unit(int i) const {  // -1: no more
+    const int g = int(gridDim.x), me = int(blockIdx.x);
+    const int mine = me < n_long ? (n_long - me + g - 1) / g : 0;
+    if (i < mine) return me + i * g;
+    int j = i - mine;
+    const int rem = n_long % g;
+    if (me >= rem) {
+      if (j < extra) return n_long + (me - rem) * extra + j;
+      j -= extra;
+    }
+    const int at = (g - rem) * extra + me + j * g;
+    return at < n_short ? n_long + at : -1;
+  }
+};
+
+template <int kProblems>
+struct GemmParams {
+  GemmProblem p[kProblems];
+  GemmDeal deal;
+  int32_t* status;
+  // the gate's and its backward's: p[0].c = h or da, then
+  CUtensorMap db, h;
+  const __nv_bfloat16* bias_up;
+  void* codes;        // checkpoint: [row tile][group][a, b][chunk of 16 bytes][128 rows], then
+  uint32_t* scales;   // [row tile][group][128 rows], bf16 of a and of b
+  float* col_sums;    // backward: [row tile][warp][2 x hidden] sums of da and db over 32 rows, or NULL
+  int32_t groups, hidden;
+  int32_t write_h;
+};
+
+struct GemmUnit {
+  int problem, row, col, begin, end, split;
+};
+template <int kProblems>
+__device__ __forceinline__ GemmUnit gemm_unit(const GemmParams<kProblems>& g, int u) {
+  GemmUnit r;
+  int i = 0;
+  if constexpr (kProblems > 1) {
+#pragma unroll 1
+    for (; i < kProblems - 1; ++i) {
+      const int n = g.p[i].row_tiles * g.p[i].col_tiles * g.p[i].splits;
+      if (u < n) break;
+      u -= n;
+    }
+  }
+  const GemmProblem& p = g.p[i];
+  r.problem = i;
+  r.split = 0;
+  if (p.splits > 1) {
+    const int tiles = p.row_tiles * p.col_tiles;
+    r.split = u / tiles;
+    u -= r.split * tiles;
+  }
+  r.row = u / p.col_tiles;
+  r.col = u - r.row * p.col_tiles;
+  r.begin = r.split * p.split_steps;
+  r.end = min(r.begin + p.split_steps, p.steps);
+  return r;
+}
+
+// ---- activations ---------------------------------------------------------------------------
+constexpr int kActSilu = 0, kActGelu = 1;
+
+// gate(a) and, for the backward, its slope.
+//   silu: a s with s = 1 / (1 + e^-a); slope s (1 + a (1 - s)).
+//   gelu: a Phi(a); slope Phi + a phi. Phi by Abramowitz and Stegun 7.1.26: with z = |a| / sqrt 2, t = 1 / (1 + 0.3275911 z),
+//   erfc(z) = t (a1 + t (a2 + t (a3 + t (a4 + t a5)))) e^-z^2, off by at most 1.5e-7; its exponential is phi's as well.
+// Both take one exponential and one reciprocal. A large negative a must give 0 and not 0 x inf: e^-a overflows to inf,
+// whose reciprocal is 0.
+template <int kAct>
+__device__ __forceinline__ float gate_of(float a) {
+  if constexpr (kAct == kActSilu) {
+    return __fdividef(1.f, 1.f + fast_exp2(a * -1.4426950408889634f)) * a;
+  } else {
+    const float z = fabsf(a) * 0.70710678118654752f;
+    const float t = __fdividef(1.f, fmaf(0.3275911f, z, 1.f));
+    const float e = fast_exp2(a * a * -0.72134752044448170f);
+    float q = fmaf(t, 1.061405429f, -1.453152027f);
+    q = fmaf(t, q, 1.421413741f);
+    q = fmaf(t, q, -0.284496736f);
+    q = fmaf(t, q, 0.254829592f) * t * 0.5f * e;  // Phi(-|a|)
+    return a * (a < 0.f ? q : 1.f - q);
+  }
+}
+template <int kAct>
+__device__ __forceinline__ void gate_and_slope(float a, float& gate, float& slope) {
+  if constexpr (kAct == kActSilu) {
+    const float s = __fdividef(1.f, 1.f + fast_exp2(a * -1.4426950408889634f));
+    gate = a * s;
+    slope = fmaf(gate, 1.f - s, s);
+  } else {
+    const float z = fabsf(a) * 0.70710678118654752f;
+    const float t = __fdividef(1.f, fmaf(0.3275911f, z, 1.f));
+    const float e = fast_exp2(a * a * -0.72134752044448170f);
+    float q = fmaf(t, 1.061405429f, -1.453152027f);
+    q = fmaf(t, q, 1.421413741f);
+    q = fmaf(t, q, -0.284496736f);
+    q = fmaf(t, q, 0.254829592f) * t * 0.5f * e;
+    const float phi = a < 0.f ? q : 1.f - q;
+    gate = a * phi;
+    slope = fmaf(a * 0.39894228040143268f, e, phi);
+  }
+}
+
+// ---- the checkpoint ------------------------------------------------------------------------
+// 32 features of a token share a scale. 16 bits: fp16 of v / 2^k with the group's largest magnitude in [2^14, 2^15), so
+// every value within 2^-29 of it keeps 11 bits (bf16 would keep 8 and cost the gradients a rounding as large as that
+// of their own operands). 8 bits: round(v / s), s = max |v| / 127 rounded up to bf16. A group with a value that is not
+// finite is NaN as a whole in 8 bits; in 16 bits its scale is 1.
+template <int kBits>
+struct Codes {
+  static constexpr int kWords = kGroup * kBits / 32;   // of a thread's 32 values
+  static constexpr int kChunks = kWords / 4;           // of 16 bytes
+};
+
+__device__ __forceinline__ float abs_max32(const float (&v)[32]) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) m = max3_nan(m, fabsf(v[i]), fabsf(v[i + 1]));
+  return m;
+}
+
+// Returns the scale as the upper half of its fp32 bits.
+template <int kBits>
+__device__ __forceinline__ uint32_t encode(const float (&v)[32], uint32_t (&w)[Codes<kBits>::kWords]) {
+  const float m = abs_max32(v);
+  if constexpr (kBits == 16) {
+    uint32_t e = __float_as_uint(m) >> 23;
+    e = e == 255u ? 141u : max(e, 15u);
+    const float inv = __uint_as_float((268u - e) << 23);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const __half2 h = __floats2half2_rn(v[2 * i] * inv, v[2 * i + 1] * inv);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return (e - 14u) << 7;
+  } else {
+    uint32_t s = (__float_as_uint(__fdiv_rn(m, 127.f)) + 0xFFFFu) >> 16;
+    float inv = __fdividef(1.f, __uint_as_float(s << 16));
+    if (!(m < __uint_as_float(0x7F800000u))) s = 0x7FC0u, inv = 0.f;   // (also NaN)
+    else if (s < 0x0D80u) s = 0u, inv = 0.f;                            // below 2^-100: zeros
+    // Adding 1.5 * 2^23 rounds to a whole number, whose low byte is the code.
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t b[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) b[k] = __float_as_uint(fmaf(v[4 * i + k], inv, 12582912.f));
+      w[i] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+    }
+    return s;
+  }
+}
+
+// Value i of the 32 (i known at compile time).
+template <int kBits>
+__device__ __forceinline__ float decode(const uint32_t (&w)[Codes<kBits>::kWords], int i, float scale) {
+  if constexpr (kBits == 16) {
+    const __half2 h = *reinterpret_cast<const __half2*>(&w[i >> 1]);
+    return ((i & 1) ? __high2float(h) : __low2float(h)) * scale;
+  } else {
+    // The code with its sign bit turned, in the low byte of 2^23: 2^23 + code + 128.
+    const uint32_t u = __byte_perm(w[i >> 2] ^ 0x80808080u, 0x4B000000u, 0x7440 | (i & 3));
+    return (__uint_as_float(u) - 8388736.f) * scale;
+  }
+}
+
+// Sum of each of 32 values over the warp's lanes; lane l receives that of value l.
+__device__ __forceinline__ float column_sums(float (&v)[32], int lane) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    const bool up = (lane & off) != 0;
+#pragma unroll
+    for (int i = 0; i < off; ++i) {
+      const float keep = up ? v[i + off] : v[i], send = up ? v[i] : v[i + off];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, off);
+    }
+  }
+  return v[0];
+}
+
+__device__ __forceinline__ void add_bias32(float (&v)[32], const __nv_bfloat16* bias, int col, int n) {
+  if (bias == nullptr) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (col + 8 * i >= n) break;  // (n is a multiple of 8)
+    const uint4 b = *reinterpret_cast<const uint4*>(bias + col + 8 * i);
+    const uint32_t u[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[8 * i + 2 * k] += __uint_as_float(u[k] << 16);
+      v[8 * i + 2 * k + 1] += __uint_as_float(u[k] & 0xFFFF0000u);
+    }
+  }
+}
+
+__device__ __forceinline__ void tmem_ld32f(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  tmem_ld32(taddr, r);
+  tmem_wait_ld();
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Eight 16-byte chunks of a 128-byte row, or four of a 64-byte row, where TMA's swizzle expects them.
+__device__ __forceinline__ void stage32_128b(uint32_t block, int row, int half, const float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    st_shared_v4(block + swz128(row, half * 4 + i), pack_bf16(v[8 * i], v[8 * i + 1]), pack_bf16(v[8 * i + 2], v[8 * i + 3]),
+                 pack_bf16(v[8 * i + 4], v[8 * i + 5]), pack_bf16(v[8 * i + 6], v[8 * i + 7]));
+}
+__device__ __forceinline__ void stage32_64b(uint32_t block, int row, const float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    st_shared_v4(block + row * 64 + ((i ^ ((row >> 1) & 3)) << 4), pack_bf16(v[8 * i], v[8 * i + 1]),
+                 pack_bf16(v[8 * i + 2], v[8 * i + 3]), pack_bf16(v[8 * i + 4], v[8 * i + 5]),
+                 pack_bf16(v[8 * i + 6], v[8 * i + 7]));
+}
+
+// ---- the kernel ----------------------------------------------------------------------------
+template <int kKind, int kAct, int kBits, int kProblems>
+__global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmParams<kProblems> g) {
+  using L = GemmSmem<kKind>;
+  constexpr int kStages = L::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t bars = base + L::kBars;
+  const uint32_t full = bars, empty = bars + 8 * kStages, acc_full = bars + 16 * kStages, acc_empty = acc_full + 16,
+                 tmem_slot = acc_empty + 16, abort_at = tmem_slot + 4;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_raw + (abort_at - smem_u32(smem_raw)));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(acc_full + 8 * i, 1), mbar_init(acc_empty + 8 * i, 8);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  pdl_wait();
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch_dependents();  // behind the allocation: the next kernel's blocks may ask for columns too
+  uint32_t tmem;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int i = 0;; ++i) {
+        const int id = g.deal.unit(i);
+        if (id < 0) break;
+        const GemmUnit u = gemm_unit(g, id);
+        const GemmProblem& p = g.p[u.problem];
+        const int cols = p.cols;
+        const uint32_t bytes = kGemmBytesA + uint32_t(cols) * (kGemmDepth * 2);
+        for (int s = u.begin; s < u.end; ++s) {
+          mbar_wait(empty + 8 * stage, phase ^ 1, abort_flag);
+          const uint32_t bar = full + 8 * stage, at_a = base + stage * kGemmStageBytes, at_b = at_a + kGemmBytesA;
+          mbar_arrive_expect_tx(bar, bytes);
+          const int second = s >= p.steps0;
+          const int k = (second ? s - p.steps0 : s) * kGemmDepth;
+          if (p.a_mn) {
+            for (int b = 0; b < 2; ++b) tma_load_2d(at_a + b * 8192, &p.a[second], bar, u.row * kGemmRows + b * 64, k);
+          } else {
+            tma_load_2d(at_a, &p.a[second], bar, k, u.row * kGemmRows);
+          }
+          if constexpr (kKind == kGemmGate) {
+            const int half = cols / 2;
+            tma_load_2d(at_b, &p.b[0], bar, k, u.col * half);
+            tma_load_2d(at_b + half * 128, &p.b[1], bar, k, u.col * half);
+          } else if (p.b_mn) {
+            for (int b = 0; b < cols / 64; ++b) tma_load_2d(at_b + b * 8192, &p.b[second], bar, u.col * cols + b * 64, k);
+          } else {
+            tma_load_2d(at_b, &p.b[second], bar, k, u.col * cols);
+          }
+          if (++stage == kStages) stage = 0, phase ^= 1;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int i = 0;; ++i) {
+        const int id = g.deal.unit(i);
+        if (id < 0) break;
+        const GemmUnit u = gemm_unit(g, id);
+        const GemmProblem& p = g.p[u.problem];
+        const uint32_t idesc = make_idesc(kGemmRows, p.cols, p.a_mn, p.b_mn);
+        const uint64_t step_a = p.a_mn ? 2048 >> 4 : 32 >> 4, step_b = p.b_mn ? 2048 >> 4 : 32 >> 4;
+        const uint32_t acc = tmem + (i & 1) * kGemmMaxCols;
+        mbar_wait(acc_empty + 8 * (i & 1), ((i >> 1) & 1) ^ 1, abort_flag);
+        tc_fence_after();
+        for (int s = u.begin; s < u.end; ++s) {
+          mbar_wait(full + 8 * stage, phase, abort_flag);
+          tc_fence_after();
+          const uint32_t at_a = base + stage * kGemmStageBytes;
+          uint64_t da = make_sdesc(at_a, 8192, 1024), db = make_sdesc(at_a + kGemmBytesA, 8192, 1024);
+#pragma unroll
+          for (int k = 0; k < kGemmDepth / 16; ++k) {
+            mma_ss(acc, da, db, idesc, s > u.begin || k > 0);
+            da += step_a, db += step_b;
+          }
+          tc_commit(empty + 8 * stage);
+          if (++stage == kStages) stage = 0, phase ^= 1;
+        }
+        tc_commit(acc_full + 8 * (i & 1));
+      }
+    }
+  } else if (warp >= 4) {
+    const int wg = (warp >> 2) - 1, row = (warp & 3) * 32 + lane;  // tensor-memory lane = row of the tile
+    const uint32_t staging = base + L::kStaging + wg * L::kStagingWg;
+    const uint32_t lanes = uint32_t(warp & 3) << 21;
+    const bool leader = (threadIdx.x & 127) == 0;
+    for (int i = 0;; ++i) {
+      const int id = g.deal.unit(i);
+      if (id < 0) break;
+      const GemmUnit u = gemm_unit(g, id);
+      const GemmProblem& p = g.p[u.problem];
+      const uint32_t acc = tmem + lanes + (i & 1) * kGemmMaxCols;
+      mbar_wait(acc_full + 8 * (i & 1), (i >> 1) & 1, abort_flag);
+      tc_fence_after();
+      if constexpr (kKind == kGemmGate) {
+        const int half = p.cols / 2, f0 = u.col * half;
+        for (int blk = wg * 64; blk < half; blk += 128) {
+          if (f0 + blk >= g.hidden) continue;
+          if (leader) bulk_wait_group_read0();
+          named_barrier(1 + wg, 128);
+#pragma unroll 1
+          for (int q = 0; q < 2; ++q) {
+            const int f = f0 + blk + q * 32;
+            if (f >= g.hidden) continue;
+            float a[32], b[32];
+            tmem_ld32f(acc + blk + q * 32, a);
+            tmem_ld32f(acc + half + blk + q * 32, b);
+            add_bias32(a, p.bias, f, g.hidden);
+            add_bias32(b, g.bias_up, f, g.hidden);
+            if constexpr (kBits > 0) {
+              constexpr int kW = Codes<kBits ? kBits : 16>::kWords, kC = kW / 4;
+              const int64_t at = int64_t(u.row) * g.groups + f / kGroup;
+              uint4* codes = static_cast<uint4*>(g.codes) + at * (2 * kC * kGemmRows) + row;
+              uint32_t w[kW];
+              uint32_t scales = encode<kBits>(a, w);
+#pragma unroll
+              for (int c = 0; c < kC; ++c)
+                codes[c * kGemmRows] = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+              scales |= encode<kBits>(b, w) << 16;
+#pragma unroll
+              for (int c = 0; c < kC; ++c)
+                codes[(kC + c) * kGemmRows] = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+              g.scales[at * kGemmRows + row] = scales;
+            }
+#pragma unroll
+            for (int k = 0; k < 32; ++k) a[k] = gate_of<kAct>(a[k]) * b[k];
+            stage32_128b(staging, row, q, a);
+          }
+          fence_proxy_async_smem();
+          named_barrier(1 + wg, 128);
+          if (leader) tma_store_2d(&p.c, staging, f0 + blk, u.row * kGemmRows), bulk_commit_group();
+        }
+      } else if constexpr (kKind == kGemmDact) {
+        constexpr int kW = Codes<kBits ? kBits : 16>::kWords, kC = kW / 4;
+        const int f0 = u.col * p.cols;
+        for (int blk = wg * 32; blk < p.cols; blk += 64) {
+          const int f = f0 + blk;
+          if (f >= g.hidden) continue;
+          const int64_t at = int64_t(u.row) * g.groups + f / kGroup;
+          const uint4* codes = static_cast<const uint4*>(g.codes) + at * (2 * kC * kGemmRows) + row;
+          uint32_t wa[kW], wb[kW];
+#pragma unroll
+          for (int c = 0; c < kC; ++c) {
+            const uint4 x = codes[c * kGemmRows], y = codes[(kC + c) * kGemmRows];
+            wa[4 * c] = x.x, wa[4 * c + 1] = x.y, wa[4 * c + 2] = x.z, wa[4 * c + 3] = x.w;
+            wb[4 * c] = y.x, wb[4 * c + 1] = y.y, wb[4 * c + 2] = y.z, wb[4 * c + 3] = y.w;
+          }
+          const uint32_t scales = g.scales[at * kGemmRows + row];
+          const float sa = __uint_as_float(scales << 16), sb = __uint_as_float(scales & 0xFFFF0000u);
+          float d[32], e[32], h[32];
+          tmem_ld32f(acc + blk, d);
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            const float a = decode<kBits>(wa, k, sa), b = decode<kBits>(wb, k, sb);
+            float gate, slope;
+            gate_and_slope<kAct>(a, gate, slope);
+            e[k] = d[k] * gate;
+            if constexpr (kBits == 8) h[k] = gate * b;
+            d[k] = d[k] * b * slope;
+          }
+          if (leader) bulk_wait_group_read0();
+          named_barrier(1 + wg, 128);
+          stage32_64b(staging, row, d);
+          stage32_64b(staging + 8192, row, e);
+          if constexpr (kBits == 8) stage32_64b(staging + 16384, row, h);
+          fence_proxy_async_smem();
+          named_barrier(1 + wg, 128);
+          if (leader) {
+            tma_store_2d(&p.c, staging, f, u.row * kGemmRows);
+            tma_store_2d(&g.db, staging + 8192, f, u.row * kGemmRows);
+            if constexpr (kBits == 8) tma_store_2d(&g.h, staging + 16384, f, u.row * kGemmRows);
+            bulk_commit_group();
+          }
+          if (g.col_sums != nullptr) {
+            float* sums = g.col_sums + (int64_t(u.row) * 4 + (warp & 3)) * (2 * int64_t(g.hidden));
+            const float sd = column_sums(d, lane), se = column_sums(e, lane);
+            if (f + lane < g.hidden) sums[f + lane] = sd, sums[g.hidden + f + lane] = se;
+          }
+        }
+      } else {
+        const int c0 = u.col * p.cols;
+        if (p.splits > 1) {
+          float4* out = reinterpret_cast<float4*>(p.partial) +
+                        ((int64_t(u.split) * p.row_tiles + u.row) * p.col_tiles + u.col) * (int64_t(p.cols) / 4 * kGemmRows) + row;
+          for (int blk = wg * 32; blk < p.cols; blk += 64) {
+            float v[32];
+            tmem_ld32f(acc + blk, v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              out[(blk / 4 + k) * kGemmRows] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+          }
+        } else {
+          for (int blk = wg * 64; blk < p.cols; blk += 128) {
+            if (c0 + blk >= p.n) continue;
+            if (leader) bulk_wait_group_read0();
+            named_barrier(1 + wg, 128);
+#pragma unroll 1
+            for (int q = 0; q < 2; ++q) {
+              float v[32];
+              tmem_ld32f(acc + blk + q * 32, v);
+              add_bias32(v, p.bias, c0 + blk + q * 32, p.n);
+              stage32_128b(staging, row, q, v);
+            }
+            fence_proxy_async_smem();
+            named_barrier(1 + wg, 128);
+            if (leader) tma_store_2d(&p.c, staging, c0 + blk, u.row * kGemmRows), bulk_commit_group();
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty + 8 * (i & 1));
+    }
+    if (leader) bulk_wait_group<0>();
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+  if (threadIdx.x == 0) report_abort(abort_flag, g.status);
+}
+
+}  // namespace nb

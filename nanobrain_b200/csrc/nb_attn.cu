@@ -13,6 +13,7 @@
 
 #include "bwd_kernel.cuh"
 #include "fwd_kernel.cuh"
+#include "host.h"
 #include "sched_kernel.cuh"
 #include "selftest_kernel.cuh"
 
@@ -720,3 +721,25 @@ int nb_attn_schedule_host(const int32_t* cu_seqlens_q, const int32_t* cu_seqlens
 }
 
 }  // extern "C"
+
+// ---- for the library's other sources (host.h) ------------------------------------------------
+int nb::host_prepare(int* sms) {
+  if (const int rc = ensure_device_ready()) return rc;
+  *sms = device_sm_count();
+  return NB_ATTN_OK;
+}
+
+int nb::host_matrix_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t cols, int64_t stride, int box_rows,
+                        int box_cols) {
+  const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
+  const cuuint64_t strides[1] = {cuuint64_t(stride) * 2};
+  const cuuint32_t box[2] = {cuuint32_t(box_cols), cuuint32_t(box_rows)};
+  const cuuint32_t elem[2] = {1, 1};
+  const EncodeTiledFn encode = get_encode();
+  if (encode == nullptr) return NB_ATTN_ERR_TENSOR_MAP;
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, elem,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? NB_ATTN_OK : NB_ATTN_ERR_TENSOR_MAP;
+}

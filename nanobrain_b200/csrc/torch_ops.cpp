@@ -12,7 +12,6 @@
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/cuda/CUDAContext.h>
-#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
@@ -36,8 +35,6 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 using Two = std::tuple<Tensor, Tensor>;
 using Three = std::tuple<Tensor, Tensor, Tensor>;
-
-constexpr int64_t kHeadDim = 64;
 
 #define NB_REQUIRE(cond, ...) TORCH_CHECK(cond, "nanobrain_b200.sdpa: ", __VA_ARGS__)
 
@@ -108,6 +105,13 @@ namespace {
 
 using nbt::after_launch;
 using nbt::check_rc;
+using nbt::dense_desc;
+using nbt::dense_layout;
+using nbt::kHeadDim;
+using nbt::new_dense;
+using nbt::new_tensor;
+using nbt::packed_desc;
+using nbt::packed_layout;
 using nbt::raise_for_status;
 using nbt::status_ptr;
 
@@ -133,43 +137,6 @@ void check_cu(const Tensor& cu, const char* name, const Tensor& like) {
   NB_REQUIRE(cu.scalar_type() == at::kInt && cu.dim() == 1 && cu.numel() >= 2, name, " must be int32 [B+1]");
   NB_REQUIRE(cu.device() == like.device(), name, " must live on the same device as the tokens");
   NB_REQUIRE(cu.is_contiguous(), name, " must be contiguous");
-}
-
-// Can the kernels address this tensor in place (head_dim contiguous, 16-byte rows)?
-bool strides_ok(const Tensor& t) {
-  const int64_t n = t.dim();
-  if (t.stride(n - 1) != 1 || (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) != 0) return false;
-  for (int64_t i = 0; i + 1 < n; ++i)
-    if (t.size(i) > 1 && (t.stride(i) <= 0 || t.stride(i) % 8 != 0)) return false;
-  return true;
-}
-
-// Logical [B, H, L, 64]: as it is, or a copy in [B, L, H, 64] memory.
-Tensor dense_layout(const Tensor& t) {
-  return strides_ok(t) ? t : t.transpose(1, 2).contiguous().transpose(1, 2);
-}
-Tensor packed_layout(const Tensor& t) { return strides_ok(t) ? t : t.contiguous(); }
-
-nb_attn_tensor dense_desc(const Tensor& t) {
-  const int64_t b = t.size(0), h = t.size(1), l = t.size(2);
-  return {t.data_ptr(), b > 1 ? t.stride(0) : h * l * kHeadDim, l > 1 ? t.stride(2) : h * kHeadDim,
-          h > 1 ? t.stride(1) : kHeadDim};
-}
-nb_attn_tensor packed_desc(const Tensor& t) {
-  const int64_t n = t.size(0), h = t.size(1);
-  return {t.data_ptr(), 0, n > 1 ? t.stride(0) : h * kHeadDim, h > 1 ? t.stride(1) : kHeadDim};
-}
-
-// Uninitialised tensors on the device of `like`, which is current here: from the caching allocator as
-// at::empty's, without its two dispatched calls (seven tensors per forward + backward).
-Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
-  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
-}
-// Logical [B, H, L, 64] in [B, L, H, 64] memory.
-Tensor new_dense(const Tensor& like) {
-  const int64_t b = like.size(0), h = like.size(1), l = like.size(2);
-  return at::detail::empty_strided_cuda({b, h, l, kHeadDim}, {l * h * kHeadDim, kHeadDim, h * kHeadDim, 1},
-                                        at::kBFloat16, like.device());
 }
 
 nb_attn_shape dense_shape(const Tensor& q, const Tensor& k, double scale) {
@@ -429,4 +396,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sdpa_varlen", &sdpa_varlen, py::call_guard<py::gil_scoped_release>());
   m.def("status_word", &status_word);
   nbt::bind_encoder(m);
+  nbt::bind_block(m);
 }
