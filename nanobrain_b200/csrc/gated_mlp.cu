@@ -161,8 +161,18 @@ __global__ void __launch_bounds__(256) split_sum_kernel(const __grid_constant__ 
 
 // Sums of a matrix' columns over chunks of kSumRows rows: a block takes 64 columns.
 constexpr int kSumRows = 512;
-__global__ void __launch_bounds__(256) col_partial_kernel(const bf16* m, int64_t stride, int64_t rows, int n, float* out) {
+struct ColPartialParams {
+  const bf16* m;
+  int64_t stride, rows;
+  float* out;
+  int32_t n;
+};
+__global__ void __launch_bounds__(256) col_partial_kernel(const __grid_constant__ ColPartialParams p) {
   __shared__ float part[32][65];
+  const bf16* m = p.m;
+  const int64_t stride = p.stride, rows = p.rows;
+  const int n = p.n;
+  float* out = p.out;
   pdl_wait();
   pdl_launch_dependents();
   const int oct = threadIdx.x & 7, lane = threadIdx.x >> 3, c = blockIdx.x * 64 + oct * 8;
@@ -222,29 +232,31 @@ __global__ void __launch_bounds__(1024) col_sum_kernel(const __grid_constant__ C
 }
 
 // ---- host --------------------------------------------------------------------------------------
-template <typename... KArgs, typename... Args>
-int launch(void (*kernel)(KArgs...), dim3 grid, unsigned threads, size_t smem, void* stream, const Args&... args) {
+template <typename Arg>
+int launch(void (*kernel)(Arg), dim3 grid, unsigned threads, size_t smem, void* stream, const Arg& arg, int cluster = 1) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = unsigned(cluster), attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? NB_ATTN_OK : NB_ATTN_ERR_LAUNCH;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, arg) == cudaSuccess ? NB_ATTN_OK : NB_ATTN_ERR_LAUNCH;
 }
 
 // A GEMM kernel needs its shared memory allowed once per device.
 constexpr int kMaxDevices = 64;
-template <int kKind, int kAct, int kBits, int kProblems>
+template <int kCtas, int kKind, int kAct, int kBits, int kProblems>
 int launch_gemm(const GemmParams<kProblems>& g, int sms, void* stream) {
   static std::mutex mutex;
   static bool ready[kMaxDevices];
-  auto* kernel = gemm_kernel<kKind, kAct, kBits, kProblems>;
-  constexpr int kSmem = GemmSmem<kKind>::kBytes;
+  auto* kernel = gemm_kernel<kCtas, kKind, kAct, kBits, kProblems>;
+  constexpr int kSmem = GemmSmem<kKind, kCtas>::kBytes;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return NB_ATTN_ERR_DEVICE;
   {
@@ -255,24 +267,41 @@ int launch_gemm(const GemmParams<kProblems>& g, int sms, void* stream) {
       ready[dev] = true;
     }
   }
-  const int units = g.deal.n_long + g.deal.n_short;
-  return launch(kernel, dim3(unsigned(std::min(units, sms))), kGemmThreads, kSmem, stream, g);
+  const int units = g.deal.n_long + g.deal.n_short, teams = std::min(units, sms / kCtas);
+  return launch(kernel, dim3(unsigned(teams * kCtas)), kGemmThreads, kSmem, stream, g, kCtas);
+}
+template <int kKind, int kAct, int kBits, int kProblems>
+int launch_gemm(const GemmParams<kProblems>& g, int ctas, int sms, void* stream) {
+  return ctas == 2 ? launch_gemm<2, kKind, kAct, kBits, kProblems>(g, sms, stream)
+                   : launch_gemm<1, kKind, kAct, kBits, kProblems>(g, sms, stream);
 }
 
 int div_up(int64_t a, int64_t b) { return int((a + b - 1) / b); }
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
-// Columns of a tile, a multiple of `unit`, by the clocks that a CTA's share of the tiles takes: a 64-deep step's MMAs
-// take two clocks a column, but not less than its operands' 128-byte reads from shared memory; a tile also costs its
-// epilogue's start.
-int tile_cols(int row_tiles, int n, int steps, int sms, int unit) {
-  int best = kGemmMaxCols;
-  double least = 0;
-  for (int cols = kGemmMaxCols; cols >= unit; cols -= unit) {
-    const int64_t tiles = int64_t(row_tiles) * div_up(n, cols);
-    const double step = std::max(2.0 * cols, 128.0 + cols);
-    const double cost = double((tiles + sms - 1) / sms) * (steps * step + 800.0);
-    if (cols == kGemmMaxCols || cost < 0.97 * least) best = cols, least = cost;
+// Teams of one or two CTAs, and the columns of their tiles, by the clocks that a team's share of the tiles takes. A 64-deep
+// step's MMAs take two clocks a column; its operands cross the port of a CTA's shared memory (128 bytes a clock) twice.
+// A tile also costs its epilogue's start and end, of which the last one of a team is not hidden.
+struct Tiling {
+  int ctas, cols, row_tiles, col_tiles;
+  double clocks;
+};
+double step_clocks(const Tiling& t) { return std::max(2.0 * t.cols, 256.0 + 2.0 * t.cols / t.ctas); }
+Tiling tiling(int64_t m, int n, int steps, int sms, int ctas, int cols) {
+  Tiling t{ctas, cols, div_up(m, int64_t(ctas) * kGemmRows), div_up(n, cols), 0.0};
+  const int64_t tiles = int64_t(t.row_tiles) * t.col_tiles, teams = sms / ctas;
+  t.clocks = double((tiles + teams - 1) / teams) * (steps * step_clocks(t) + 400.0) + 2.0 * cols + 1000.0 * ctas;
+  return t;
+}
+// Widths are multiples of 64 per CTA, and of `unit`.
+Tiling best_tiling(int64_t m, int n, int steps, int sms, int unit) {
+  Tiling best = tiling(m, n, steps, sms, 2, kGemmMaxCols);
+  for (int ctas = 2; ctas >= 1; --ctas) {
+    const int by = std::max(unit, 64 * ctas);
+    for (int cols = kGemmMaxCols; cols >= by; cols -= by) {
+      const Tiling t = tiling(m, n, steps, sms, ctas, cols);
+      if (t.clocks < 0.98 * best.clocks) best = t;
+    }
   }
   return best;
 }
@@ -341,35 +370,69 @@ int launch_few(const nb_gated_mlp_fwd_args& a, void* stream) {
 }
 
 template <int kKind, int kAct>
-int launch_bits(const GemmParams<1>& g, int checkpoint, int sms, void* stream) {
+int launch_bits(const GemmParams<1>& g, int checkpoint, int ctas, int sms, void* stream) {
   switch (checkpoint) {
-    case NB_CHECKPOINT_16BIT: return launch_gemm<kKind, kAct, 16, 1>(g, sms, stream);
-    case NB_CHECKPOINT_8BIT: return launch_gemm<kKind, kAct, 8, 1>(g, sms, stream);
+    case NB_CHECKPOINT_16BIT: return launch_gemm<kKind, kAct, 16, 1>(g, ctas, sms, stream);
+    case NB_CHECKPOINT_8BIT: return launch_gemm<kKind, kAct, 8, 1>(g, ctas, sms, stream);
   }
-  if constexpr (kKind == kGemmGate) return launch_gemm<kKind, kAct, 0, 1>(g, sms, stream);
+  if constexpr (kKind == kGemmGate) return launch_gemm<kKind, kAct, 0, 1>(g, ctas, sms, stream);
   return NB_ATTN_ERR_SHAPE;
 }
 template <int kKind>
-int launch_act(const GemmParams<1>& g, const nb_gated_mlp_shape& s, int sms, void* stream) {
-  return s.activation == NB_ACT_SILU ? launch_bits<kKind, kActSilu>(g, s.checkpoint, sms, stream)
-                                     : launch_bits<kKind, kActGelu>(g, s.checkpoint, sms, stream);
+int launch_act(const GemmParams<1>& g, const nb_gated_mlp_shape& s, int ctas, int sms, void* stream) {
+  return s.activation == NB_ACT_SILU ? launch_bits<kKind, kActSilu>(g, s.checkpoint, ctas, sms, stream)
+                                     : launch_bits<kKind, kActGelu>(g, s.checkpoint, ctas, sms, stream);
 }
 
-void set_tiles(GemmProblem* p, int64_t rows, int n, int cols_of_tile, int per_tile, int steps0, int steps) {
-  p->n = n;
-  p->row_tiles = div_up(rows, kGemmRows);
-  p->cols = cols_of_tile;
-  p->col_tiles = div_up(n, per_tile);
+void set_tiles(GemmProblem* p, int64_t rows, int n, const Tiling& t, int steps0, int steps) {
+  p->m = int(rows), p->n = n;
+  p->row_tiles = t.row_tiles, p->col_tiles = t.col_tiles, p->cols = t.cols;
   p->steps0 = steps0, p->steps = steps;
   p->splits = 1, p->split_steps = steps;
 }
 
-// Where the backward's scratch lies in the workspace, and how the weight gradients are cut.
+// Where the backward's scratch lies in the workspace, and how the products behind it are cut.
 struct BwdPlan {
   size_t da, db, h, col_sums, dy_sums, parts[3], bytes;
-  int cols[3], splits[3], split_steps[3];  // of dWg, dWu, dWd
-  int dx_cols;
+  Tiling dx, dw[3];                // dw: of Wg, Wu, Wd
+  int splits[3], split_steps[3];
+  double clocks;
 };
+
+// The products behind da and db by teams of `ctas`; parts[] receives the bytes that are needed there.
+BwdPlan plan_products(BwdPlan p, const nb_gated_mlp_bwd_args& a, int sms, int ctas) {
+  const nb_gated_mlp_shape& s = a.shape;
+  const int dx_steps = 2 * div_up(s.hidden, kGemmDepth), dw_steps = div_up(s.tokens, kGemmDepth), unit = 64 * ctas;
+  const bool wanted[3] = {a.d_w_gate.ptr != nullptr, a.d_w_up.ptr != nullptr, a.d_w_down.ptr != nullptr};
+  const auto width = [unit](int n) { return std::min(kGemmMaxCols, div_up(div_up(n, div_up(n, kGemmMaxCols)), unit) * unit); };
+  p.dx = tiling(s.tokens, s.dim, dx_steps, sms, ctas, width(s.dim));
+  double total = 0.0, longest = 0.0;
+  if (a.dx.ptr != nullptr) {
+    longest = step_clocks(p.dx) * dx_steps;
+    total = longest * p.dx.row_tiles * p.dx.col_tiles;
+  }
+  for (int i = 0; i < 3; ++i) {
+    const int m = i < 2 ? s.hidden : s.dim, n = i < 2 ? s.dim : s.hidden;
+    p.dw[i] = tiling(m, n, dw_steps, sms, ctas, width(n));
+    if (wanted[i]) total += step_clocks(p.dw[i]) * p.dw[i].row_tiles * p.dw[i].col_tiles * dw_steps;
+  }
+  // A weight gradient's unit runs over all tokens. Where that is more than a team's even share of the launch's work, it is
+  // cut into parts of about half a share, which are added up behind (fp32, in a fixed order).
+  const double share = total / (sms / ctas);
+  for (int i = 0; i < 3; ++i) {
+    const double steps = share / step_clocks(p.dw[i]);
+    int splits = 1;
+    if (dw_steps > 0.8 * steps) splits = std::min(div_up(dw_steps, 8), int(dw_steps / std::max(0.5 * steps, 8.0)) + 1);
+    splits = std::max(1, std::min(splits, 32));
+    p.split_steps[i] = div_up(dw_steps, splits);
+    p.splits[i] = div_up(dw_steps, p.split_steps[i]);
+    const size_t tiles = size_t(p.dw[i].row_tiles) * ctas * p.dw[i].col_tiles;
+    p.parts[i] = wanted[i] && p.splits[i] > 1 ? tiles * p.dw[i].cols * kGemmRows * 4 * p.splits[i] : 0;
+    if (wanted[i]) longest = std::max(longest, step_clocks(p.dw[i]) * p.split_steps[i]);
+  }
+  p.clocks = std::max(share + 0.25 * longest, longest) + 1000.0 * ctas;
+  return p;
+}
 
 BwdPlan plan_bwd(const nb_gated_mlp_bwd_args& a, int sms) {
   const nb_gated_mlp_shape& s = a.shape;
@@ -383,33 +446,16 @@ BwdPlan plan_bwd(const nb_gated_mlp_bwd_args& a, int sms) {
   const size_t hidden_bytes = size_t(s.tokens) * s.hidden * 2;
   p.da = take(hidden_bytes), p.db = take(hidden_bytes);
   p.h = take(s.checkpoint == NB_CHECKPOINT_8BIT ? hidden_bytes : 0);
-  const int row_tiles = div_up(s.tokens, kGemmRows);
-  p.col_sums = take(a.d_b_gate != nullptr || a.d_b_up != nullptr ? size_t(row_tiles) * 4 * 2 * s.hidden * 4 : 0);
+  const size_t row_tiles = size_t(div_up(s.tokens, kGemmRows));
+  p.col_sums = take(a.d_b_gate != nullptr || a.d_b_up != nullptr ? row_tiles * 4 * 2 * s.hidden * 4 : 0);
   p.dy_sums = take(a.d_b_down != nullptr ? size_t(div_up(s.tokens, kSumRows)) * s.dim * 4 : 0);
-  // A weight gradient's unit runs over all tokens. Where that is more than a CTA's even share of the launch's work, it is
-  // cut into parts of about half a share, which are added up behind (fp32, in a fixed order).
-  const int dx_steps = 2 * div_up(s.hidden, kGemmDepth), dw_steps = div_up(s.tokens, kGemmDepth);
-  const bool wanted[3] = {a.d_w_gate.ptr != nullptr, a.d_w_up.ptr != nullptr, a.d_w_down.ptr != nullptr};
-  p.dx_cols = tile_cols(row_tiles, s.dim, dx_steps, sms, 64);
-  double total = a.dx.ptr != nullptr ? double(row_tiles) * div_up(s.dim, p.dx_cols) * p.dx_cols * dx_steps : 0.0;
-  for (int i = 0; i < 3; ++i) {
-    const int rows = i < 2 ? s.hidden : s.dim, n = i < 2 ? s.dim : s.hidden;
-    p.cols[i] = (div_up(n, div_up(n, kGemmMaxCols)) + 63) / 64 * 64;
-    if (wanted[i]) total += double(div_up(rows, kGemmRows)) * div_up(n, p.cols[i]) * p.cols[i] * dw_steps;
-  }
-  for (int i = 0; i < 3; ++i) {
-    const int rows = i < 2 ? s.hidden : s.dim, n = i < 2 ? s.dim : s.hidden;
-    const double share = total / sms / p.cols[i];  // in steps
-    int splits = 1;
-    if (dw_steps > 0.8 * share) splits = std::min(div_up(dw_steps, 8), int(dw_steps / std::max(0.5 * share, 8.0)) + 1);
-    splits = std::max(1, std::min(splits, 32));
-    p.split_steps[i] = div_up(dw_steps, splits);
-    p.splits[i] = div_up(dw_steps, p.split_steps[i]);
-    const size_t tiles = size_t(div_up(rows, kGemmRows)) * div_up(n, p.cols[i]);
-    p.parts[i] = take(wanted[i] && p.splits[i] > 1 ? tiles * p.cols[i] * kGemmRows * 4 * p.splits[i] : 0);
-  }
-  p.bytes = std::max<size_t>(at, 256);
-  return p;
+  // All products of the launch have teams of one size.
+  BwdPlan best = plan_products(p, a, sms, 2);
+  const BwdPlan single = plan_products(p, a, sms, 1);
+  if (single.clocks < 0.98 * best.clocks) best = single;
+  for (int i = 0; i < 3; ++i) best.parts[i] = take(best.parts[i]);
+  best.bytes = std::max<size_t>(at, 256);
+  return best;
 }
 
 }  // namespace
@@ -440,11 +486,14 @@ extern "C" int nb_gated_mlp_fwd(const nb_gated_mlp_fwd_args* args, void* stream)
   if (s.checkpoint == NB_CHECKPOINT_NONE && s.tokens <= kFewTokens)
     return s.activation == NB_ACT_SILU ? launch_few<kActSilu>(*args, stream) : launch_few<kActGelu>(*args, stream);
 
-  const int row_tiles = div_up(s.tokens, kGemmRows), steps = div_up(s.dim, kGemmDepth);
+  const int steps = div_up(s.dim, kGemmDepth);
   GemmParams<1> g{};
   GemmProblem& p = g.p[0];
-  const int cols = tile_cols(row_tiles, 2 * s.hidden, steps, sms, 128);
-  set_tiles(&p, s.tokens, s.hidden, cols, cols / 2, steps, steps);
+  // (a tile has as many columns of a as of b, 64 at least)
+  const Tiling tg = best_tiling(s.tokens, 2 * s.hidden, steps, sms, 128);
+  const int cols = tg.cols;
+  set_tiles(&p, s.tokens, s.hidden, tg, steps, steps);
+  p.col_tiles = div_up(s.hidden, cols / 2);
   NB_TRY(map_k_major(&p.a[0], args->x, s.tokens, s.dim, kGemmRows));
   NB_TRY(map_k_major(&p.b[0], args->w_gate, s.hidden, s.dim, cols / 2));
   NB_TRY(map_k_major(&p.b[1], args->w_up, s.hidden, s.dim, cols / 2));
@@ -459,16 +508,17 @@ extern "C" int nb_gated_mlp_fwd(const nb_gated_mlp_fwd_args* args, void* stream)
 
   GemmParams<1> d{};
   GemmProblem& q = d.p[0];
-  const int down_steps = div_up(s.hidden, kGemmDepth), down_cols = tile_cols(row_tiles, s.dim, down_steps, sms, 64);
-  set_tiles(&q, s.tokens, s.dim, down_cols, down_cols, down_steps, down_steps);
+  const int down_steps = div_up(s.hidden, kGemmDepth);
+  const Tiling td = best_tiling(s.tokens, s.dim, down_steps, sms, 64);
+  set_tiles(&q, s.tokens, s.dim, td, down_steps, down_steps);
   NB_TRY(map_k_major(&q.a[0], args->h, s.tokens, s.hidden, kGemmRows));
-  NB_TRY(map_k_major(&q.b[0], args->w_down, s.dim, s.hidden, down_cols));
+  NB_TRY(map_k_major(&q.b[0], args->w_down, s.dim, s.hidden, td.cols / td.ctas));
   NB_TRY(host_matrix_map(&q.c, args->y.ptr, s.tokens, s.dim, args->y.stride, kGemmRows, 64));
   q.bias = static_cast<const bf16*>(args->b_down);
   d.deal.n_short = q.row_tiles * q.col_tiles;
   d.status = args->status;
-  NB_TRY(launch_act<kGemmGate>(g, s, sms, stream));
-  return launch_gemm<kGemmPlain, 0, 0, 1>(d, sms, stream);
+  NB_TRY(launch_act<kGemmGate>(g, s, tg.ctas, sms, stream));
+  return launch_gemm<kGemmPlain, 0, 0, 1>(d, td.ctas, sms, stream);
 }
 
 extern "C" size_t nb_gated_mlp_bwd_workspace_bytes(const nb_gated_mlp_bwd_args* args) {
@@ -511,11 +561,13 @@ extern "C" int nb_gated_mlp_bwd(const nb_gated_mlp_bwd_args* args, void* stream)
                             a.d_b_gate != nullptr || a.d_b_up != nullptr;
   const bool dact = hidden_grads || (a.d_w_down.ptr != nullptr && s.checkpoint == NB_CHECKPOINT_8BIT);
   GemmParams<1> act{};
+  Tiling act_tiling{};
   if (dact) {
     GemmParams<1>& g = act;
     GemmProblem& p = g.p[0];
-    const int steps = div_up(s.dim, kGemmDepth), cols = tile_cols(row_tiles, s.hidden, steps, sms, 64);
-    set_tiles(&p, s.tokens, s.hidden, cols, cols, steps, steps);
+    const int steps = div_up(s.dim, kGemmDepth);
+    act_tiling = best_tiling(s.tokens, s.hidden, steps, sms, 64);
+    set_tiles(&p, s.tokens, s.hidden, act_tiling, steps, steps);
     p.b_mn = 1;
     NB_TRY(map_k_major(&p.a[0], a.dy, s.tokens, s.dim, kGemmRows));
     NB_TRY(map_mn_major(&p.b[0], a.w_down, s.dim, s.hidden));
@@ -539,7 +591,7 @@ extern "C" int nb_gated_mlp_bwd(const nb_gated_mlp_bwd_args* args, void* stream)
   const auto add_dx = [&]() -> int {
     if (a.dx.ptr == nullptr) return NB_ATTN_OK;
     GemmProblem& p = g.p[n++];
-    set_tiles(&p, s.tokens, s.dim, plan.dx_cols, plan.dx_cols, hidden_steps, 2 * hidden_steps);
+    set_tiles(&p, s.tokens, s.dim, plan.dx, hidden_steps, 2 * hidden_steps);
     p.b_mn = 1;
     NB_TRY(map_k_major(&p.a[0], da, s.tokens, s.hidden, kGemmRows));
     NB_TRY(map_k_major(&p.a[1], db, s.tokens, s.hidden, kGemmRows));
@@ -553,7 +605,7 @@ extern "C" int nb_gated_mlp_bwd(const nb_gated_mlp_bwd_args* args, void* stream)
     if (out.ptr == nullptr) return NB_ATTN_OK;
     GemmProblem& p = g.p[n++];
     const int rows = which < 2 ? s.hidden : s.dim, cols = which < 2 ? s.dim : s.hidden;
-    set_tiles(&p, rows, cols, plan.cols[which], plan.cols[which], dw_steps, dw_steps);
+    set_tiles(&p, rows, cols, plan.dw[which], dw_steps, dw_steps);
     p.a_mn = p.b_mn = 1;
     p.splits = plan.splits[which], p.split_steps = plan.split_steps[which];
     NB_TRY(map_mn_major(&p.a[0], left, s.tokens, rows));
@@ -564,9 +616,9 @@ extern "C" int nb_gated_mlp_bwd(const nb_gated_mlp_bwd_args* args, void* stream)
       SplitItem& i = sums.item[sums.n_items++];
       i.partial = reinterpret_cast<const float4*>(p.partial);
       i.out = static_cast<bf16*>(out.ptr), i.stride = out.stride;
-      i.rows = rows, i.n = cols, i.row_tiles = p.row_tiles, i.col_tiles = p.col_tiles, i.cols = p.cols;
+      i.rows = rows, i.n = cols, i.row_tiles = p.row_tiles * plan.dx.ctas, i.col_tiles = p.col_tiles, i.cols = p.cols;
       i.splits = p.splits;
-      i.pieces = int64_t(p.row_tiles) * p.col_tiles * (p.cols / 8) * kGemmRows;
+      i.pieces = int64_t(i.row_tiles) * p.col_tiles * (p.cols / 8) * kGemmRows;
       return NB_ATTN_OK;
     }
     return host_matrix_map(&p.c, out.ptr, rows, cols, out.stride, kGemmRows, 64);
@@ -578,17 +630,17 @@ extern "C" int nb_gated_mlp_bwd(const nb_gated_mlp_bwd_args* args, void* stream)
   NB_TRY(add_dw(1, db, a.x, a.d_w_up));
   NB_TRY(add_dw(2, a.dy, h, a.d_w_down));
   if (dw_first) NB_TRY(add_dx());
-  if (dact) NB_TRY(launch_act<kGemmDact>(act, s, sms, stream));
+  if (dact) NB_TRY(launch_act<kGemmDact>(act, s, act_tiling.ctas, sms, stream));
   if (n > 0) {
     const int n_long = dw_first ? dw_units : dx_units, n_short = dw_first ? dx_units : dw_units;
     g.deal.n_long = n_long, g.deal.n_short = n_short;
-    const int grid = std::min(n_long + n_short, sms), rem = n_long % grid;
+    const int teams = std::min(n_long + n_short, sms / plan.dx.ctas), rem = n_long % teams;
     if (n_short > 0 && rem > 0) {
       const int dw_len = plan.split_steps[0], dx_len = 2 * hidden_steps;
       const int ratio = dw_first ? dw_len / dx_len : dx_len / std::max(1, dw_len);
-      g.deal.extra = std::min(ratio, n_short / (grid - rem));
+      g.deal.extra = std::min(ratio, n_short / (teams - rem));
     }
-    NB_TRY((launch_gemm<kGemmPlain, 0, 0, 4>(g, sms, stream)));
+    NB_TRY((launch_gemm<kGemmPlain, 0, 0, 4>(g, plan.dx.ctas, sms, stream)));
   }
   if (sums.n_items > 0) {
     int64_t pieces = 0;
@@ -608,8 +660,8 @@ extern "C" int nb_gated_mlp_bwd(const nb_gated_mlp_bwd_args* args, void* stream)
   if (a.d_b_down != nullptr) {
     float* dy_sums = reinterpret_cast<float*>(ws + plan.dy_sums);
     const int chunks = div_up(s.tokens, kSumRows);
-    NB_TRY(launch(col_partial_kernel, dim3(div_up(s.dim, 64), chunks), 256, 0, stream, static_cast<const bf16*>(a.dy.ptr),
-                  a.dy.stride, s.tokens, int(s.dim), dy_sums));
+    NB_TRY(launch(col_partial_kernel, dim3(div_up(s.dim, 64), chunks), 256, 0, stream,
+                  ColPartialParams{static_cast<const bf16*>(a.dy.ptr), a.dy.stride, s.tokens, dy_sums, s.dim}));
     add_col(a.d_b_down, dy_sums, s.dim, chunks, s.dim);
   }
   if (cols.n_items > 0) {

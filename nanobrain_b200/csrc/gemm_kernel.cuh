@@ -10,8 +10,9 @@
 // along memory the tile is a K-major operand, otherwise an MN-major one, so no product needs a transposed copy.
 // Accumulators are two sets of 256 tensor-memory columns: the epilogue of a unit runs under the products of the next.
 //
-// 128 x 256 columns because both operands come from shared memory: a 16-deep MMA takes 128 clocks and reads 12 KB, 96
-// clocks of the shared-memory port; 128 x 128 would read 8 KB in 64.
+// Large products are made by pairs of CTAs (cta_group::2) on tiles of 256 rows x 256 columns: each CTA loads its 128 rows
+// of A and half of B. What bounds one CTA's 128 x 256 tile is its shared memory's port (128 bytes a clock): a 64-deep
+// step takes 512 clocks of MMAs, but its 48 KB are written once and read once, 768 clocks. A pair's CTA moves 32 KB.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -23,17 +24,17 @@ namespace nb {
 constexpr int kGemmRows = 128, kGemmDepth = 64, kGemmMaxCols = 256;
 constexpr int kGemmThreads = 384;
 constexpr int kGemmBytesA = kGemmRows * kGemmDepth * 2, kGemmBytesB = kGemmMaxCols * kGemmDepth * 2;
-constexpr int kGemmStageBytes = kGemmBytesA + kGemmBytesB;
 constexpr int kGroup = 32;  // features of a token that share a scale in the checkpoint
 
 enum GemmKind { kGemmGate = 0, kGemmDact = 1, kGemmPlain = 2 };
 
 // Shared memory: stages, then the epilogue's staging (a part per warpgroup), then barriers.
-template <int kKind>
+template <int kKind, int kCtas>
 struct GemmSmem {
-  static constexpr int kStages = kKind == kGemmDact ? 3 : 4;
+  static constexpr int kStageBytes = kGemmBytesA + kGemmBytesB / kCtas;
+  static constexpr int kStages = kCtas == 2 ? (kKind == kGemmDact ? 5 : 6) : (kKind == kGemmDact ? 3 : 4);
   static constexpr int kStagingWg = kKind == kGemmDact ? 3 * 8192 : 16384;
-  static constexpr int kStaging = kStages * kGemmStageBytes;
+  static constexpr int kStaging = kStages * kStageBytes;
   static constexpr int kBars = kStaging + 2 * kStagingWg;
   static constexpr int kBytes = kBars + 256 + 1024;  // (+ 1024: the base is aligned by hand)
 };
@@ -42,20 +43,21 @@ struct GemmProblem {
   CUtensorMap a[2], b[2], c;  // a, b: of the two ranges of steps (gate: b of Wg and Wu)
   const __nv_bfloat16* bias;  // per column, or NULL
   float* partial;             // [split][row tile][column tile][columns / 4][128 rows][4], where splits > 1
-  int32_t n;                  // columns of the output
-  int32_t row_tiles, col_tiles, cols;  // cols: of a tile
+  int32_t m, n;               // rows and columns of the output
+  int32_t row_tiles, col_tiles, cols;  // tiles of 128 rows per CTA of the team; cols: of a tile
   int32_t steps0, steps;      // 64-deep steps of the first range, of both
   int32_t splits, split_steps;
   int32_t a_mn, b_mn;         // the operand's inner index does not run along memory
 };
 
-// The units of a launch, dealt to the CTAs in a fixed manner: `n_long` units (the problems with more steps come first
-// in the list) in turns; the CTAs left with one long unit fewer then take `extra` short ones each, and the rest of
-// the short units goes round again.
+// The units of a launch, dealt to the teams (CTAs or pairs) in a fixed manner: `n_long` units (the problems with more
+// steps come first in the list) in turns; the teams left with one long unit fewer then take `extra` short ones each, and
+// the rest of the short units goes round again.
 struct GemmDeal {
   int32_t n_long, n_short, extra;
+  template <int kCtas>
   __device__ __forceinline__ int unit(int i) const {  // -1: no more
-    const int g = int(gridDim.x), me = int(blockIdx.x);
+    const int g = int(gridDim.x) / kCtas, me = int(blockIdx.x) / kCtas;
     const int mine = me < n_long ? (n_long - me + g - 1) / g : 0;
     if (i < mine) return me + i * g;
     int j = i - mine;
@@ -273,10 +275,11 @@ __device__ __forceinline__ void stage32_64b(uint32_t block, int row, const float
 }
 
 // ---- the kernel ----------------------------------------------------------------------------
-template <int kKind, int kAct, int kBits, int kProblems>
+template <int kCtas, int kKind, int kAct, int kBits, int kProblems>
 __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmParams<kProblems> g) {
-  using L = GemmSmem<kKind>;
+  using L = GemmSmem<kKind, kCtas>;
   constexpr int kStages = L::kStages;
+  constexpr bool kPair = kCtas == 2;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t bars = base + L::kBars;
@@ -284,20 +287,23 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                  tmem_slot = acc_empty + 16, abort_at = tmem_slot + 4;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_raw + (abort_at - smem_u32(smem_raw)));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = kPair ? int(cluster_rank()) : 0;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
-    for (int i = 0; i < 2; ++i) mbar_init(acc_full + 8 * i, 1), mbar_init(acc_empty + 8 * i, 8);
+    for (int i = 0; i < 2; ++i) mbar_init(acc_full + 8 * i, 1), mbar_init(acc_empty + 8 * i, 8 * kCtas);
     *abort_flag = 0;
     fence_mbar_init();
   }
   pdl_wait();
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
+    if constexpr (kPair) tmem_alloc_pair(tmem_slot, 512), tmem_relinquish_pair();
+    else tmem_alloc(tmem_slot, 512), tmem_relinquish();
     tc_fence_before();
   }
-  __syncthreads();
+  __syncwarp();
+  if constexpr (kPair) cluster_sync();  // the other CTA's barriers are there
+  else __syncthreads();
   tc_fence_after();
   pdl_launch_dependents();  // behind the allocation: the next kernel's blocks may ask for columns too
   uint32_t tmem;
@@ -305,49 +311,67 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
 
   if (warp == 0) {
     if (lane == 0) {
+      const auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+        if constexpr (kPair) tma_load_2d_pair(dst, map, bar, c0, c1);
+        else tma_load_2d(dst, map, bar, c0, c1);
+      };
       int stage = 0;
       uint32_t phase = 0;
       for (int i = 0;; ++i) {
-        const int id = g.deal.unit(i);
+        const int id = g.deal.template unit<kCtas>(i);
         if (id < 0) break;
         const GemmUnit u = gemm_unit(g, id);
         const GemmProblem& p = g.p[u.problem];
-        const int cols = p.cols;
-        const uint32_t bytes = kGemmBytesA + uint32_t(cols) * (kGemmDepth * 2);
+        const int cols = p.cols, mine = cols / kCtas;  // columns of the tile, and those that this CTA loads
+        const int row0 = (u.row * kCtas + rank) * kGemmRows, col0 = u.col * cols + rank * mine;
+        const uint32_t bytes = kCtas * (kGemmBytesA + uint32_t(mine) * (kGemmDepth * 2));
         for (int s = u.begin; s < u.end; ++s) {
           mbar_wait(empty + 8 * stage, phase ^ 1, abort_flag);
-          const uint32_t bar = full + 8 * stage, at_a = base + stage * kGemmStageBytes, at_b = at_a + kGemmBytesA;
-          mbar_arrive_expect_tx(bar, bytes);
+          const uint32_t at_a = base + stage * L::kStageBytes, at_b = at_a + kGemmBytesA;
+          uint32_t bar = full + 8 * stage;
+          if (rank == 0) mbar_arrive_expect_tx(bar, bytes);  // (of both CTAs: all loads count on rank 0's barrier)
+          if constexpr (kPair) bar = map_to_rank(bar, 0);
           const int second = s >= p.steps0;
           const int k = (second ? s - p.steps0 : s) * kGemmDepth;
           if (p.a_mn) {
-            for (int b = 0; b < 2; ++b) tma_load_2d(at_a + b * 8192, &p.a[second], bar, u.row * kGemmRows + b * 64, k);
+            for (int b = 0; b < 2; ++b) load(at_a + b * 8192, &p.a[second], bar, row0 + b * 64, k);
           } else {
-            tma_load_2d(at_a, &p.a[second], bar, k, u.row * kGemmRows);
+            load(at_a, &p.a[second], bar, k, row0);
           }
           if constexpr (kKind == kGemmGate) {
+            // Columns of a, then as many of b: in a pair rank 0 holds those of a and rank 1 those of b.
             const int half = cols / 2;
-            tma_load_2d(at_b, &p.b[0], bar, k, u.col * half);
-            tma_load_2d(at_b + half * 128, &p.b[1], bar, k, u.col * half);
+            if constexpr (kPair) {
+              load(at_b, &p.b[rank], bar, k, u.col * half);
+            } else {
+              load(at_b, &p.b[0], bar, k, u.col * half);
+              load(at_b + half * 128, &p.b[1], bar, k, u.col * half);
+            }
           } else if (p.b_mn) {
-            for (int b = 0; b < cols / 64; ++b) tma_load_2d(at_b + b * 8192, &p.b[second], bar, u.col * cols + b * 64, k);
+            for (int b = 0; b < mine / 64; ++b) load(at_b + b * 8192, &p.b[second], bar, col0 + b * 64, k);
           } else {
-            tma_load_2d(at_b, &p.b[second], bar, k, u.col * cols);
+            load(at_b, &p.b[second], bar, k, col0);
           }
+          if (++stage == kStages) stage = 0, phase ^= 1;
+        }
+      }
+      if constexpr (kPair) {  // rank 0's arrivals on this CTA's barriers are in before it may end
+        for (int s = 0; s < kStages; ++s) {
+          mbar_wait(empty + 8 * stage, phase ^ 1, abort_flag);
           if (++stage == kStages) stage = 0, phase ^= 1;
         }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       int stage = 0;
       uint32_t phase = 0;
       for (int i = 0;; ++i) {
-        const int id = g.deal.unit(i);
+        const int id = g.deal.template unit<kCtas>(i);
         if (id < 0) break;
         const GemmUnit u = gemm_unit(g, id);
         const GemmProblem& p = g.p[u.problem];
-        const uint32_t idesc = make_idesc(kGemmRows, p.cols, p.a_mn, p.b_mn);
+        const uint32_t idesc = make_idesc(kGemmRows * kCtas, p.cols, p.a_mn, p.b_mn);
         const uint64_t step_a = p.a_mn ? 2048 >> 4 : 32 >> 4, step_b = p.b_mn ? 2048 >> 4 : 32 >> 4;
         const uint32_t acc = tmem + (i & 1) * kGemmMaxCols;
         mbar_wait(acc_empty + 8 * (i & 1), ((i >> 1) & 1) ^ 1, abort_flag);
@@ -355,17 +379,20 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         for (int s = u.begin; s < u.end; ++s) {
           mbar_wait(full + 8 * stage, phase, abort_flag);
           tc_fence_after();
-          const uint32_t at_a = base + stage * kGemmStageBytes;
+          const uint32_t at_a = base + stage * L::kStageBytes;
           uint64_t da = make_sdesc(at_a, 8192, 1024), db = make_sdesc(at_a + kGemmBytesA, 8192, 1024);
 #pragma unroll
           for (int k = 0; k < kGemmDepth / 16; ++k) {
-            mma_ss(acc, da, db, idesc, s > u.begin || k > 0);
+            if constexpr (kPair) mma_ss_pair(acc, da, db, idesc, s > u.begin || k > 0);
+            else mma_ss(acc, da, db, idesc, s > u.begin || k > 0);
             da += step_a, db += step_b;
           }
-          tc_commit(empty + 8 * stage);
+          if constexpr (kPair) tc_commit_pair(empty + 8 * stage);
+          else tc_commit(empty + 8 * stage);
           if (++stage == kStages) stage = 0, phase ^= 1;
         }
-        tc_commit(acc_full + 8 * (i & 1));
+        if constexpr (kPair) tc_commit_pair(acc_full + 8 * (i & 1));
+        else tc_commit(acc_full + 8 * (i & 1));
       }
     }
   } else if (warp >= 4) {
@@ -373,15 +400,19 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     const uint32_t staging = base + L::kStaging + wg * L::kStagingWg;
     const uint32_t lanes = uint32_t(warp & 3) << 21;
     const bool leader = (threadIdx.x & 127) == 0;
+    const uint32_t acc_free = kPair ? map_to_rank(acc_empty, 0) : acc_empty;  // where the MMAs' issuer waits
     for (int i = 0;; ++i) {
-      const int id = g.deal.unit(i);
+      const int id = g.deal.template unit<kCtas>(i);
       if (id < 0) break;
       const GemmUnit u = gemm_unit(g, id);
       const GemmProblem& p = g.p[u.problem];
       const uint32_t acc = tmem + lanes + (i & 1) * kGemmMaxCols;
       mbar_wait(acc_full + 8 * (i & 1), (i >> 1) & 1, abort_flag);
       tc_fence_after();
-      if constexpr (kKind == kGemmGate) {
+      const int row_tile = u.row * kCtas + rank, row0 = row_tile * kGemmRows;
+      if (kPair && row0 >= p.m) {
+        // the pair's second half lies behind the last row
+      } else if constexpr (kKind == kGemmGate) {
         const int half = p.cols / 2, f0 = u.col * half;
         for (int blk = wg * 64; blk < half; blk += 128) {
           if (f0 + blk >= g.hidden) continue;
@@ -398,7 +429,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             add_bias32(b, g.bias_up, f, g.hidden);
             if constexpr (kBits > 0) {
               constexpr int kW = Codes<kBits ? kBits : 16>::kWords, kC = kW / 4;
-              const int64_t at = int64_t(u.row) * g.groups + f / kGroup;
+              const int64_t at = int64_t(row_tile) * g.groups + f / kGroup;
               uint4* codes = static_cast<uint4*>(g.codes) + at * (2 * kC * kGemmRows) + row;
               uint32_t w[kW];
               uint32_t scales = encode<kBits>(a, w);
@@ -417,7 +448,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
           }
           fence_proxy_async_smem();
           named_barrier(1 + wg, 128);
-          if (leader) tma_store_2d(&p.c, staging, f0 + blk, u.row * kGemmRows), bulk_commit_group();
+          if (leader) tma_store_2d(&p.c, staging, f0 + blk, row0), bulk_commit_group();
         }
       } else if constexpr (kKind == kGemmDact) {
         constexpr int kW = Codes<kBits ? kBits : 16>::kWords, kC = kW / 4;
@@ -425,7 +456,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         for (int blk = wg * 32; blk < p.cols; blk += 64) {
           const int f = f0 + blk;
           if (f >= g.hidden) continue;
-          const int64_t at = int64_t(u.row) * g.groups + f / kGroup;
+          const int64_t at = int64_t(row_tile) * g.groups + f / kGroup;
           const uint4* codes = static_cast<const uint4*>(g.codes) + at * (2 * kC * kGemmRows) + row;
           uint32_t wa[kW], wb[kW];
 #pragma unroll
@@ -455,13 +486,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
           fence_proxy_async_smem();
           named_barrier(1 + wg, 128);
           if (leader) {
-            tma_store_2d(&p.c, staging, f, u.row * kGemmRows);
-            tma_store_2d(&g.db, staging + 8192, f, u.row * kGemmRows);
-            if constexpr (kBits == 8) tma_store_2d(&g.h, staging + 16384, f, u.row * kGemmRows);
+            tma_store_2d(&p.c, staging, f, row0);
+            tma_store_2d(&g.db, staging + 8192, f, row0);
+            if constexpr (kBits == 8) tma_store_2d(&g.h, staging + 16384, f, row0);
             bulk_commit_group();
           }
           if (g.col_sums != nullptr) {
-            float* sums = g.col_sums + (int64_t(u.row) * 4 + (warp & 3)) * (2 * int64_t(g.hidden));
+            float* sums = g.col_sums + (int64_t(row_tile) * 4 + (warp & 3)) * (2 * int64_t(g.hidden));
             const float sd = column_sums(d, lane), se = column_sums(e, lane);
             if (f + lane < g.hidden) sums[f + lane] = sd, sums[g.hidden + f + lane] = se;
           }
@@ -470,7 +501,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         const int c0 = u.col * p.cols;
         if (p.splits > 1) {
           float4* out = reinterpret_cast<float4*>(p.partial) +
-                        ((int64_t(u.split) * p.row_tiles + u.row) * p.col_tiles + u.col) * (int64_t(p.cols) / 4 * kGemmRows) + row;
+                        ((int64_t(u.split) * p.row_tiles * kCtas + row_tile) * p.col_tiles + u.col) * (int64_t(p.cols) / 4 * kGemmRows) + row;
           for (int blk = wg * 32; blk < p.cols; blk += 64) {
             float v[32];
             tmem_ld32f(acc + blk, v);
@@ -492,24 +523,30 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             }
             fence_proxy_async_smem();
             named_barrier(1 + wg, 128);
-            if (leader) tma_store_2d(&p.c, staging, c0 + blk, u.row * kGemmRows), bulk_commit_group();
+            if (leader) tma_store_2d(&p.c, staging, c0 + blk, row0), bulk_commit_group();
           }
         }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty + 8 * (i & 1));
+      if (lane == 0) {
+        if constexpr (kPair) mbar_arrive_cluster(acc_free + 8 * (i & 1));
+        else mbar_arrive(acc_free + 8 * (i & 1));
+      }
     }
     if (leader) bulk_wait_group<0>();
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  if (threadIdx.x == 0) report_abort(abort_flag, g.status);
+  __syncwarp();
+  if constexpr (kPair) cluster_sync();  // nothing of this CTA is used by the other one any more
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    if constexpr (kPair) tmem_dealloc_pair(tmem, 512);
+    else tmem_dealloc(tmem, 512);
   }
-  if (threadIdx.x == 0) report_abort(abort_flag, g.status);
 }
 
 }  // namespace nb
