@@ -256,7 +256,7 @@ int launch_gemm(const GemmParams<kProblems>& g, int sms, void* stream) {
   static std::mutex mutex;
   static bool ready[kMaxDevices];
   auto* kernel = gemm_kernel<kCtas, kKind, kAct, kBits, kProblems>;
-  constexpr int kSmem = GemmSmem<kKind, kCtas>::kBytes;
+  constexpr int kSmem = GemmSmem<kKind, kBits, kCtas>::kBytes;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return NB_ATTN_ERR_DEVICE;
   {
@@ -326,8 +326,8 @@ int check_shape(const nb_gated_mlp_shape& s) {
 }
 
 size_t code_bytes(const nb_gated_mlp_shape& s) {
-  const size_t blocks = size_t(div_up(s.tokens, kGemmRows)) * div_up(s.hidden, kGroup);
-  return blocks * kGemmRows * kGroup * 2 * (s.checkpoint == NB_CHECKPOINT_8BIT ? 1 : 2);
+  const size_t blocks = size_t(div_up(s.tokens, kGemmRows)) * div_up(s.hidden, kGroup) * 4;
+  return blocks * (s.checkpoint == NB_CHECKPOINT_8BIT ? CodeBlock<8>::kBytes : CodeBlock<16>::kBytes);
 }
 
 // Boxes of an operand whose inner index runs along memory: 64 deep x rows; of the others: 64 x 64.
@@ -462,8 +462,7 @@ BwdPlan plan_bwd(const nb_gated_mlp_bwd_args& a, int sms) {
 
 extern "C" size_t nb_gated_mlp_checkpoint_bytes(const nb_gated_mlp_shape* shape) {
   if (shape == nullptr || check_shape(*shape) != NB_ATTN_OK || shape->checkpoint == NB_CHECKPOINT_NONE) return 0;
-  const size_t scales = size_t(div_up(shape->tokens, kGemmRows)) * div_up(shape->hidden, kGroup) * kGemmRows * 4;
-  return code_bytes(*shape) + scales;
+  return code_bytes(*shape);
 }
 
 extern "C" int nb_gated_mlp_fwd(const nb_gated_mlp_fwd_args* args, void* stream) {
@@ -497,11 +496,10 @@ extern "C" int nb_gated_mlp_fwd(const nb_gated_mlp_fwd_args* args, void* stream)
   NB_TRY(map_k_major(&p.a[0], args->x, s.tokens, s.dim, kGemmRows));
   NB_TRY(map_k_major(&p.b[0], args->w_gate, s.hidden, s.dim, cols / 2));
   NB_TRY(map_k_major(&p.b[1], args->w_up, s.hidden, s.dim, cols / 2));
-  NB_TRY(host_matrix_map(&p.c, args->h.ptr, s.tokens, s.hidden, args->h.stride, kGemmRows, 64));
+  NB_TRY(host_matrix_map(&p.c, args->h.ptr, s.tokens, s.hidden, args->h.stride, 32, kGroup));
   p.bias = static_cast<const bf16*>(args->b_gate);
   g.bias_up = static_cast<const bf16*>(args->b_up);
-  g.codes = args->checkpoint;
-  g.scales = reinterpret_cast<uint32_t*>(static_cast<char*>(args->checkpoint) + code_bytes(s));
+  g.codes = static_cast<uint8_t*>(args->checkpoint);
   g.groups = div_up(s.hidden, kGroup), g.hidden = s.hidden;
   g.deal.n_short = p.row_tiles * p.col_tiles;
   g.status = args->status;
@@ -513,7 +511,7 @@ extern "C" int nb_gated_mlp_fwd(const nb_gated_mlp_fwd_args* args, void* stream)
   set_tiles(&q, s.tokens, s.dim, td, down_steps, down_steps);
   NB_TRY(map_k_major(&q.a[0], args->h, s.tokens, s.hidden, kGemmRows));
   NB_TRY(map_k_major(&q.b[0], args->w_down, s.dim, s.hidden, td.cols / td.ctas));
-  NB_TRY(host_matrix_map(&q.c, args->y.ptr, s.tokens, s.dim, args->y.stride, kGemmRows, 64));
+  NB_TRY(host_matrix_map(&q.c, args->y.ptr, s.tokens, s.dim, args->y.stride, 32, 64));
   q.bias = static_cast<const bf16*>(args->b_down);
   d.deal.n_short = q.row_tiles * q.col_tiles;
   d.status = args->status;
@@ -571,12 +569,11 @@ extern "C" int nb_gated_mlp_bwd(const nb_gated_mlp_bwd_args* args, void* stream)
     p.b_mn = 1;
     NB_TRY(map_k_major(&p.a[0], a.dy, s.tokens, s.dim, kGemmRows));
     NB_TRY(map_mn_major(&p.b[0], a.w_down, s.dim, s.hidden));
-    NB_TRY(host_matrix_map(&p.c, da.ptr, s.tokens, s.hidden, da.stride, kGemmRows, kGroup));
-    NB_TRY(host_matrix_map(&g.db, db.ptr, s.tokens, s.hidden, db.stride, kGemmRows, kGroup));
+    NB_TRY(host_matrix_map(&p.c, da.ptr, s.tokens, s.hidden, da.stride, 32, kGroup));
+    NB_TRY(host_matrix_map(&g.db, db.ptr, s.tokens, s.hidden, db.stride, 32, kGroup));
     if (s.checkpoint == NB_CHECKPOINT_8BIT)
-      NB_TRY(host_matrix_map(&g.h, h.ptr, s.tokens, s.hidden, h.stride, kGemmRows, kGroup));
-    g.codes = const_cast<void*>(a.checkpoint);
-    g.scales = reinterpret_cast<uint32_t*>(static_cast<char*>(g.codes) + code_bytes(s));
+      NB_TRY(host_matrix_map(&g.h, h.ptr, s.tokens, s.hidden, h.stride, 32, kGroup));
+    g.codes = static_cast<uint8_t*>(const_cast<void*>(a.checkpoint));
     g.groups = div_up(s.hidden, kGroup), g.hidden = s.hidden;
     if (a.d_b_gate != nullptr || a.d_b_up != nullptr) g.col_sums = reinterpret_cast<float*>(ws + plan.col_sums);
     g.deal.n_short = p.row_tiles * p.col_tiles;
@@ -598,7 +595,7 @@ extern "C" int nb_gated_mlp_bwd(const nb_gated_mlp_bwd_args* args, void* stream)
     NB_TRY(map_mn_major(&p.b[0], a.w_gate, s.hidden, s.dim));
     NB_TRY(map_mn_major(&p.b[1], a.w_up, s.hidden, s.dim));
     dx_units = p.row_tiles * p.col_tiles;
-    return host_matrix_map(&p.c, a.dx.ptr, s.tokens, s.dim, a.dx.stride, kGemmRows, 64);
+    return host_matrix_map(&p.c, a.dx.ptr, s.tokens, s.dim, a.dx.stride, 32, 64);
   };
   SplitParams sums{};
   const auto add_dw = [&](int which, const nb_matrix& left, const nb_matrix& right, const nb_matrix& out) -> int {
@@ -621,7 +618,7 @@ extern "C" int nb_gated_mlp_bwd(const nb_gated_mlp_bwd_args* args, void* stream)
       i.pieces = int64_t(i.row_tiles) * p.col_tiles * (p.cols / 8) * kGemmRows;
       return NB_ATTN_OK;
     }
-    return host_matrix_map(&p.c, out.ptr, rows, cols, out.stride, kGemmRows, 64);
+    return host_matrix_map(&p.c, out.ptr, rows, cols, out.stride, 32, 64);
   };
   // The longer units first.
   const bool dw_first = std::max({plan.split_steps[0], plan.split_steps[1], plan.split_steps[2]}) >= 2 * hidden_steps;

@@ -28,15 +28,29 @@ constexpr int kGroup = 32;  // features of a token that share a scale in the che
 
 enum GemmKind { kGemmGate = 0, kGemmDact = 1, kGemmPlain = 2 };
 
-// Shared memory: stages, then the epilogue's staging (a part per warpgroup), then barriers.
-template <int kKind, int kCtas>
+// A warp's 32 rows x 32 features of a and b in the checkpoint: [a, b][chunk of 16 bytes][row], then a word of both scales
+// (bf16) per row. Contiguous, so a bulk copy moves it.
+template <int kBits>
+struct CodeBlock {
+  static constexpr int kWords = kGroup * kBits / 32;  // of a lane's 32 values
+  static constexpr int kChunks = kWords / 4;          // of 16 bytes
+  static constexpr int kScales = 2 * kChunks * 512;   // where they begin
+  static constexpr int kBytes = kBits ? kScales + 128 : 0;
+};
+
+// Shared memory: stages, then a part for every epilogue warp (what it hands to TMA, and code blocks), then barriers.
+constexpr int kEpilogueWarps = 8;
+template <int kKind, int kBits, int kCtas>
 struct GemmSmem {
   static constexpr int kStageBytes = kGemmBytesA + kGemmBytesB / kCtas;
-  static constexpr int kStages = kCtas == 2 ? (kKind == kGemmDact ? 5 : 6) : (kKind == kGemmDact ? 3 : 4);
-  static constexpr int kStagingWg = kKind == kGemmDact ? 3 * 8192 : 16384;
-  static constexpr int kStaging = kStages * kStageBytes;
-  static constexpr int kBars = kStaging + 2 * kStagingWg;
-  static constexpr int kBytes = kBars + 256 + 1024;  // (+ 1024: the base is aligned by hand)
+  static constexpr int kTiles = kKind == kGemmPlain ? 4096 : kKind == kGemmGate ? 2048 : (kBits == 8 ? 3 : 2) * 2048;
+  static constexpr int kCodes = kKind == kGemmDact ? 2 : 1;  // code blocks
+  static constexpr int kWarpBytes = (kTiles + kCodes * CodeBlock<kBits>::kBytes + 1023) / 1024 * 1024;
+  static constexpr int kMost = 232448 - 1024 - 512 - kEpilogueWarps * kWarpBytes;
+  static constexpr int kStages = kMost / kStageBytes < 6 ? kMost / kStageBytes : 6;
+  static constexpr int kWarps = kStages * kStageBytes;
+  static constexpr int kBars = kWarps + kEpilogueWarps * kWarpBytes;
+  static constexpr int kBytes = kBars + 512 + 1024;  // (+ 1024: the base is aligned by hand)
 };
 
 struct GemmProblem {
@@ -79,8 +93,7 @@ struct GemmParams {
   // the gate's and its backward's: p[0].c = h or da, then
   CUtensorMap db, h;
   const __nv_bfloat16* bias_up;
-  void* codes;        // checkpoint: [row tile][group][a, b][chunk of 16 bytes][128 rows], then
-  uint32_t* scales;   // [row tile][group][128 rows], bf16 of a and of b
+  uint8_t* codes;     // checkpoint: [row tile][group][warp] code blocks
   float* col_sums;    // backward: [row tile][warp][2 x hidden] sums of da and db over 32 rows, or NULL
   int32_t groups, hidden;
   int32_t write_h;
@@ -165,12 +178,6 @@ __device__ __forceinline__ void gate_and_slope(float a, float& gate, float& slop
 // every value within 2^-29 of it keeps 11 bits (bf16 would keep 8 and cost the gradients a rounding as large as that
 // of their own operands). 8 bits: round(v / s), s = max |v| / 127 rounded up to bf16. A group with a value that is not
 // finite is NaN as a whole in 8 bits; in 16 bits its scale is 1.
-template <int kBits>
-struct Codes {
-  static constexpr int kWords = kGroup * kBits / 32;   // of a thread's 32 values
-  static constexpr int kChunks = kWords / 4;           // of 16 bytes
-};
-
 __device__ __forceinline__ float abs_max32(const float (&v)[32]) {
   float m = 0.f;
 #pragma unroll
@@ -180,7 +187,7 @@ __device__ __forceinline__ float abs_max32(const float (&v)[32]) {
 
 // Returns the scale as the upper half of its fp32 bits.
 template <int kBits>
-__device__ __forceinline__ uint32_t encode(const float (&v)[32], uint32_t (&w)[Codes<kBits>::kWords]) {
+__device__ __forceinline__ uint32_t encode(const float (&v)[32], uint32_t (&w)[CodeBlock<kBits>::kWords]) {
   const float m = abs_max32(v);
   if constexpr (kBits == 16) {
     uint32_t e = __float_as_uint(m) >> 23;
@@ -211,7 +218,7 @@ __device__ __forceinline__ uint32_t encode(const float (&v)[32], uint32_t (&w)[C
 
 // Value i of the 32 (i known at compile time).
 template <int kBits>
-__device__ __forceinline__ float decode(const uint32_t (&w)[Codes<kBits>::kWords], int i, float scale) {
+__device__ __forceinline__ float decode(const uint32_t (&w)[CodeBlock<kBits>::kWords], int i, float scale) {
   if constexpr (kBits == 16) {
     const __half2 h = *reinterpret_cast<const __half2*>(&w[i >> 1]);
     return ((i & 1) ? __high2float(h) : __low2float(h)) * scale;
@@ -259,32 +266,38 @@ __device__ __forceinline__ void tmem_ld32f(uint32_t taddr, float (&v)[32]) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// Eight 16-byte chunks of a 128-byte row, or four of a 64-byte row, where TMA's swizzle expects them.
-__device__ __forceinline__ void stage32_128b(uint32_t block, int row, int half, const float (&v)[32]) {
+// 32 values of a row of a box that TMA stores, 64 columns (`half` of it) or 32 wide: the chunks of 16 bytes where its
+// swizzle over 128 or 64 bytes expects them.
+__device__ __forceinline__ void stage_half_row(uint32_t box, int row, int half, const float (&v)[32]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    st_shared_v4(block + swz128(row, half * 4 + i), pack_bf16(v[8 * i], v[8 * i + 1]), pack_bf16(v[8 * i + 2], v[8 * i + 3]),
+    st_shared_v4(box + swz128(row, half * 4 + i), pack_bf16(v[8 * i], v[8 * i + 1]), pack_bf16(v[8 * i + 2], v[8 * i + 3]),
                  pack_bf16(v[8 * i + 4], v[8 * i + 5]), pack_bf16(v[8 * i + 6], v[8 * i + 7]));
 }
-__device__ __forceinline__ void stage32_64b(uint32_t block, int row, const float (&v)[32]) {
+__device__ __forceinline__ void stage_row(uint32_t box, int row, const float (&v)[32]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    st_shared_v4(block + row * 64 + ((i ^ ((row >> 1) & 3)) << 4), pack_bf16(v[8 * i], v[8 * i + 1]),
+    st_shared_v4(box + row * 64 + ((i ^ ((row >> 1) & 3)) << 4), pack_bf16(v[8 * i], v[8 * i + 1]),
                  pack_bf16(v[8 * i + 2], v[8 * i + 3]), pack_bf16(v[8 * i + 4], v[8 * i + 5]),
                  pack_bf16(v[8 * i + 6], v[8 * i + 7]));
+}
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
 }
 
 // ---- the kernel ----------------------------------------------------------------------------
 template <int kCtas, int kKind, int kAct, int kBits, int kProblems>
 __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmParams<kProblems> g) {
-  using L = GemmSmem<kKind, kCtas>;
+  using L = GemmSmem<kKind, kBits, kCtas>;
   constexpr int kStages = L::kStages;
   constexpr bool kPair = kCtas == 2;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t bars = base + L::kBars;
   const uint32_t full = bars, empty = bars + 8 * kStages, acc_full = bars + 16 * kStages, acc_empty = acc_full + 16,
-                 tmem_slot = acc_empty + 16, abort_at = tmem_slot + 4;
+                 codes_full = acc_empty + 16, tmem_slot = codes_full + 16 * kEpilogueWarps, abort_at = tmem_slot + 4;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_raw + (abort_at - smem_u32(smem_raw)));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = kPair ? int(cluster_rank()) : 0;
@@ -292,6 +305,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
     for (int i = 0; i < 2; ++i) mbar_init(acc_full + 8 * i, 1), mbar_init(acc_empty + 8 * i, 8 * kCtas);
+    if constexpr (kKind == kGemmDact)
+      for (int i = 0; i < 2 * kEpilogueWarps; ++i) mbar_init(codes_full + 8 * i, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -396,11 +411,45 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
       }
     }
   } else if (warp >= 4) {
-    const int wg = (warp >> 2) - 1, row = (warp & 3) * 32 + lane;  // tensor-memory lane = row of the tile
-    const uint32_t staging = base + L::kStaging + wg * L::kStagingWg;
-    const uint32_t lanes = uint32_t(warp & 3) << 21;
-    const bool leader = (threadIdx.x & 127) == 0;
+    // A warp works by itself on its 32 rows: it takes every other 32 (plain: 64) columns, hands boxes of 32 rows to TMA
+    // and waits for nobody. Its lane is the row. (With boxes of 128 rows, four warps met at two barriers per box, and the
+    // proxy fence waited for the checkpoint's plain stores: together 38 % of the gate epilogue's time.)
+    const int wg = (warp >> 2) - 1, quarter = warp & 3;
+    const uint32_t box = base + L::kWarps + (warp - 4) * L::kWarpBytes, block = box + L::kTiles;
+    const uint32_t lanes = uint32_t(quarter) << 21;
     const uint32_t acc_free = kPair ? map_to_rank(acc_empty, 0) : acc_empty;  // where the MMAs' issuer waits
+    constexpr int kB = kBits ? kBits : 16;
+    using Block = CodeBlock<kB>;
+    const auto rows_of = [&](const GemmUnit& u) { return (u.row * kCtas + rank) * kGemmRows; };
+    const auto code_block = [&](const GemmUnit& u, int f) {
+      return g.codes + ((int64_t(u.row * kCtas + rank) * g.groups + f / kGroup) * 4 + quarter) * Block::kBytes;
+    };
+
+    // The backward's code blocks arrive two pieces ahead of their use.
+    [[maybe_unused]] struct { int i, blk; GemmUnit u; bool live; } ahead{-1, 0, {}, true};
+    [[maybe_unused]] uint32_t piece = 0;
+    [[maybe_unused]] const uint32_t my_codes = codes_full + 16 * (warp - 4);
+    [[maybe_unused]] const auto request = [&](uint32_t slot) {  // the next piece's
+      if constexpr (kKind == kGemmDact) {
+        const int cols = g.p[0].cols;
+        ahead.blk += 64;
+        while (ahead.live && (ahead.i < 0 || ahead.blk >= cols || ahead.u.col * cols + ahead.blk >= g.hidden ||
+                              (kPair && rows_of(ahead.u) >= g.p[0].m))) {
+          const int id = g.deal.template unit<kCtas>(++ahead.i);
+          ahead.live = id >= 0;
+          if (ahead.live) ahead.u = gemm_unit(g, id);
+          ahead.blk = wg * 32;
+        }
+        if (ahead.live && lane == 0) {
+          mbar_arrive_expect_tx(my_codes + 8 * slot, Block::kBytes);
+          bulk_load(block + slot * Block::kBytes, code_block(ahead.u, ahead.u.col * cols + ahead.blk), Block::kBytes,
+                    my_codes + 8 * slot);
+        }
+      }
+    };
+    request(0);
+    request(1);
+
     for (int i = 0;; ++i) {
       const int id = g.deal.template unit<kCtas>(i);
       if (id < 0) break;
@@ -409,90 +458,91 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
       const uint32_t acc = tmem + lanes + (i & 1) * kGemmMaxCols;
       mbar_wait(acc_full + 8 * (i & 1), (i >> 1) & 1, abort_flag);
       tc_fence_after();
-      const int row_tile = u.row * kCtas + rank, row0 = row_tile * kGemmRows;
+      const int row0 = rows_of(u), row = row0 + quarter * 32;  // of the tile, of the warp
       if (kPair && row0 >= p.m) {
         // the pair's second half lies behind the last row
       } else if constexpr (kKind == kGemmGate) {
-        const int half = p.cols / 2, f0 = u.col * half;
-        for (int blk = wg * 64; blk < half; blk += 128) {
-          if (f0 + blk >= g.hidden) continue;
-          if (leader) bulk_wait_group_read0();
-          named_barrier(1 + wg, 128);
+        const int half = p.cols / 2;
 #pragma unroll 1
-          for (int q = 0; q < 2; ++q) {
-            const int f = f0 + blk + q * 32;
-            if (f >= g.hidden) continue;
-            float a[32], b[32];
-            tmem_ld32f(acc + blk + q * 32, a);
-            tmem_ld32f(acc + half + blk + q * 32, b);
-            add_bias32(a, p.bias, f, g.hidden);
-            add_bias32(b, g.bias_up, f, g.hidden);
-            if constexpr (kBits > 0) {
-              constexpr int kW = Codes<kBits ? kBits : 16>::kWords, kC = kW / 4;
-              const int64_t at = int64_t(row_tile) * g.groups + f / kGroup;
-              uint4* codes = static_cast<uint4*>(g.codes) + at * (2 * kC * kGemmRows) + row;
-              uint32_t w[kW];
-              uint32_t scales = encode<kBits>(a, w);
+        for (int blk = wg * 32; blk < half; blk += 64) {
+          const int f = u.col * half + blk;
+          if (f >= g.hidden) break;
+          float a[32], b[32];
+          tmem_ld32f(acc + blk, a);
+          tmem_ld32f(acc + half + blk, b);
+          add_bias32(a, p.bias, f, g.hidden);
+          add_bias32(b, g.bias_up, f, g.hidden);
+          if (lane == 0) bulk_wait_group_read0();  // the boxes in front have left
+          __syncwarp();
+          if constexpr (kBits > 0) {
+            uint32_t w[Block::kWords];
+            uint32_t scales = encode<kB>(a, w);
 #pragma unroll
-              for (int c = 0; c < kC; ++c)
-                codes[c * kGemmRows] = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
-              scales |= encode<kBits>(b, w) << 16;
+            for (int c = 0; c < Block::kChunks; ++c)
+              st_shared_v4(block + c * 512 + lane * 16, w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+            scales |= encode<kB>(b, w) << 16;
 #pragma unroll
-              for (int c = 0; c < kC; ++c)
-                codes[(kC + c) * kGemmRows] = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
-              g.scales[at * kGemmRows + row] = scales;
-            }
-#pragma unroll
-            for (int k = 0; k < 32; ++k) a[k] = gate_of<kAct>(a[k]) * b[k];
-            stage32_128b(staging, row, q, a);
+            for (int c = 0; c < Block::kChunks; ++c)
+              st_shared_v4(block + (Block::kChunks + c) * 512 + lane * 16, w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(block + Block::kScales + lane * 4), "r"(scales) : "memory");
           }
+#pragma unroll
+          for (int k = 0; k < 32; ++k) a[k] = gate_of<kAct>(a[k]) * b[k];
+          stage_row(box, lane, a);
           fence_proxy_async_smem();
-          named_barrier(1 + wg, 128);
-          if (leader) tma_store_2d(&p.c, staging, f0 + blk, row0), bulk_commit_group();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&p.c, box, f, row);
+            if constexpr (kBits > 0) bulk_store(code_block(u, f), block, Block::kBytes);
+            bulk_commit_group();
+          }
         }
       } else if constexpr (kKind == kGemmDact) {
-        constexpr int kW = Codes<kBits ? kBits : 16>::kWords, kC = kW / 4;
-        const int f0 = u.col * p.cols;
+#pragma unroll 1
         for (int blk = wg * 32; blk < p.cols; blk += 64) {
-          const int f = f0 + blk;
-          if (f >= g.hidden) continue;
-          const int64_t at = int64_t(row_tile) * g.groups + f / kGroup;
-          const uint4* codes = static_cast<const uint4*>(g.codes) + at * (2 * kC * kGemmRows) + row;
-          uint32_t wa[kW], wb[kW];
+          const int f = u.col * p.cols + blk;
+          if (f >= g.hidden) break;
+          const uint32_t slot = piece & 1, codes = block + slot * Block::kBytes;
+          mbar_wait(my_codes + 8 * slot, (piece >> 1) & 1, abort_flag);
+          uint32_t wa[Block::kWords], wb[Block::kWords], scales;
 #pragma unroll
-          for (int c = 0; c < kC; ++c) {
-            const uint4 x = codes[c * kGemmRows], y = codes[(kC + c) * kGemmRows];
+          for (int c = 0; c < Block::kChunks; ++c) {
+            const uint4 x = ld_shared_v4(codes + c * 512 + lane * 16),
+                        y = ld_shared_v4(codes + (Block::kChunks + c) * 512 + lane * 16);
             wa[4 * c] = x.x, wa[4 * c + 1] = x.y, wa[4 * c + 2] = x.z, wa[4 * c + 3] = x.w;
             wb[4 * c] = y.x, wb[4 * c + 1] = y.y, wb[4 * c + 2] = y.z, wb[4 * c + 3] = y.w;
           }
-          const uint32_t scales = g.scales[at * kGemmRows + row];
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(scales) : "r"(codes + Block::kScales + lane * 4) : "memory");
+          __syncwarp();
+          request(slot);
+          ++piece;
           const float sa = __uint_as_float(scales << 16), sb = __uint_as_float(scales & 0xFFFF0000u);
           float d[32], e[32], h[32];
           tmem_ld32f(acc + blk, d);
 #pragma unroll
           for (int k = 0; k < 32; ++k) {
-            const float a = decode<kBits>(wa, k, sa), b = decode<kBits>(wb, k, sb);
+            const float a = decode<kB>(wa, k, sa), b = decode<kB>(wb, k, sb);
             float gate, slope;
             gate_and_slope<kAct>(a, gate, slope);
             e[k] = d[k] * gate;
             if constexpr (kBits == 8) h[k] = gate * b;
             d[k] = d[k] * b * slope;
           }
-          if (leader) bulk_wait_group_read0();
-          named_barrier(1 + wg, 128);
-          stage32_64b(staging, row, d);
-          stage32_64b(staging + 8192, row, e);
-          if constexpr (kBits == 8) stage32_64b(staging + 16384, row, h);
+          if (lane == 0) bulk_wait_group_read0();
+          __syncwarp();
+          stage_row(box, lane, d);
+          stage_row(box + 2048, lane, e);
+          if constexpr (kBits == 8) stage_row(box + 4096, lane, h);
           fence_proxy_async_smem();
-          named_barrier(1 + wg, 128);
-          if (leader) {
-            tma_store_2d(&p.c, staging, f, row0);
-            tma_store_2d(&g.db, staging + 8192, f, row0);
-            if constexpr (kBits == 8) tma_store_2d(&g.h, staging + 16384, f, row0);
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&p.c, box, f, row);
+            tma_store_2d(&g.db, box + 2048, f, row);
+            if constexpr (kBits == 8) tma_store_2d(&g.h, box + 4096, f, row);
             bulk_commit_group();
           }
           if (g.col_sums != nullptr) {
-            float* sums = g.col_sums + (int64_t(row_tile) * 4 + (warp & 3)) * (2 * int64_t(g.hidden));
+            float* sums = g.col_sums + (int64_t(row0 / kGemmRows) * 4 + quarter) * (2 * int64_t(g.hidden));
             const float sd = column_sums(d, lane), se = column_sums(e, lane);
             if (f + lane < g.hidden) sums[f + lane] = sd, sums[g.hidden + f + lane] = se;
           }
@@ -501,7 +551,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         const int c0 = u.col * p.cols;
         if (p.splits > 1) {
           float4* out = reinterpret_cast<float4*>(p.partial) +
-                        ((int64_t(u.split) * p.row_tiles * kCtas + row_tile) * p.col_tiles + u.col) * (int64_t(p.cols) / 4 * kGemmRows) + row;
+                        ((int64_t(u.split) * p.row_tiles * kCtas + row0 / kGemmRows) * p.col_tiles + u.col) *
+                            (int64_t(p.cols) / 4 * kGemmRows) + quarter * 32 + lane;
+#pragma unroll 1
           for (int blk = wg * 32; blk < p.cols; blk += 64) {
             float v[32];
             tmem_ld32f(acc + blk, v);
@@ -510,20 +562,21 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
               out[(blk / 4 + k) * kGemmRows] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
           }
         } else {
-          for (int blk = wg * 64; blk < p.cols; blk += 128) {
-            if (c0 + blk >= p.n) continue;
-            if (leader) bulk_wait_group_read0();
-            named_barrier(1 + wg, 128);
 #pragma unroll 1
+          for (int blk = wg * 64; blk < p.cols; blk += 128) {
+            if (c0 + blk >= p.n) break;
+            if (lane == 0) bulk_wait_group_read0();
+            __syncwarp();
+#pragma unroll
             for (int q = 0; q < 2; ++q) {
               float v[32];
               tmem_ld32f(acc + blk + q * 32, v);
               add_bias32(v, p.bias, c0 + blk + q * 32, p.n);
-              stage32_128b(staging, row, q, v);
+              stage_half_row(box, lane, q, v);
             }
             fence_proxy_async_smem();
-            named_barrier(1 + wg, 128);
-            if (leader) tma_store_2d(&p.c, staging, c0 + blk, row0), bulk_commit_group();
+            __syncwarp();
+            if (lane == 0) tma_store_2d(&p.c, box, c0 + blk, row), bulk_commit_group();
           }
         }
       }
@@ -534,7 +587,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         else mbar_arrive(acc_free + 8 * (i & 1));
       }
     }
-    if (leader) bulk_wait_group<0>();
+    if (lane == 0) bulk_wait_group<0>();
   }
   __syncwarp();
   tc_fence_before();
