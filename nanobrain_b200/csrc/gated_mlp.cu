@@ -256,7 +256,8 @@ int launch_gemm(const GemmParams<kProblems>& g, int sms, void* stream) {
   static std::mutex mutex;
   static bool ready[kMaxDevices];
   auto* kernel = gemm_kernel<kCtas, kKind, kAct, kBits, kProblems>;
-  constexpr int kSmem = GemmSmem<kKind, kBits, kCtas>::kBytes;
+  using L = GemmLayout<kKind, kBits, kCtas>;
+  constexpr int kSmem = L::kBytes;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return NB_ATTN_ERR_DEVICE;
   {
@@ -268,7 +269,7 @@ int launch_gemm(const GemmParams<kProblems>& g, int sms, void* stream) {
     }
   }
   const int units = g.deal.n_long + g.deal.n_short, teams = std::min(units, sms / kCtas);
-  return launch(kernel, dim3(unsigned(teams * kCtas)), kGemmThreads, kSmem, stream, g, kCtas);
+  return launch(kernel, dim3(unsigned(teams * kCtas)), L::kThreads, kSmem, stream, g, kCtas);
 }
 template <int kKind, int kAct, int kBits, int kProblems>
 int launch_gemm(const GemmParams<kProblems>& g, int ctas, int sms, void* stream) {
@@ -277,6 +278,8 @@ int launch_gemm(const GemmParams<kProblems>& g, int ctas, int sms, void* stream)
 }
 
 int div_up(int64_t a, int64_t b) { return int((a + b - 1) / b); }
+// Rows of hidden features in scratch begin on lines of 128 bytes.
+int64_t padded(int hidden) { return (int64_t(hidden) + 63) / 64 * 64; }
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Teams of one or two CTAs, and the columns of their tiles, by the clocks that a team's share of the tiles takes. A 64-deep
@@ -443,7 +446,7 @@ BwdPlan plan_bwd(const nb_gated_mlp_bwd_args& a, int sms) {
     at += align256(n);
     return here;
   };
-  const size_t hidden_bytes = size_t(s.tokens) * s.hidden * 2;
+  const size_t hidden_bytes = size_t(s.tokens) * padded(s.hidden) * 2;
   p.da = take(hidden_bytes), p.db = take(hidden_bytes);
   p.h = take(s.checkpoint == NB_CHECKPOINT_8BIT ? hidden_bytes : 0);
   const size_t row_tiles = size_t(div_up(s.tokens, kGemmRows));
@@ -475,6 +478,8 @@ extern "C" int nb_gated_mlp_fwd(const nb_gated_mlp_fwd_args* args, void* stream)
   NB_TRY(check_matrix(args->w_down, s.hidden));
   NB_TRY(check_matrix(args->y, s.dim));
   NB_TRY(check_matrix(args->h, s.hidden));
+  // (16 values at a time are written there)
+  if ((reinterpret_cast<uintptr_t>(args->h.ptr) & 31u) != 0 || args->h.stride % 16 != 0) return NB_ATTN_ERR_ALIGN;
   for (const void* b : {args->b_gate, args->b_up, args->b_down}) NB_TRY(check_bias(b));
   if (s.checkpoint != NB_CHECKPOINT_NONE) {
     if (args->checkpoint == nullptr) return NB_ATTN_ERR_NULL;
@@ -496,7 +501,7 @@ extern "C" int nb_gated_mlp_fwd(const nb_gated_mlp_fwd_args* args, void* stream)
   NB_TRY(map_k_major(&p.a[0], args->x, s.tokens, s.dim, kGemmRows));
   NB_TRY(map_k_major(&p.b[0], args->w_gate, s.hidden, s.dim, cols / 2));
   NB_TRY(map_k_major(&p.b[1], args->w_up, s.hidden, s.dim, cols / 2));
-  NB_TRY(host_matrix_map(&p.c, args->h.ptr, s.tokens, s.hidden, args->h.stride, 32, kGroup));
+  g.h = static_cast<bf16*>(args->h.ptr), g.stride = args->h.stride;
   p.bias = static_cast<const bf16*>(args->b_gate);
   g.bias_up = static_cast<const bf16*>(args->b_up);
   g.codes = static_cast<uint8_t*>(args->checkpoint);
@@ -550,8 +555,9 @@ extern "C" int nb_gated_mlp_bwd(const nb_gated_mlp_bwd_args* args, void* stream)
   const BwdPlan plan = plan_bwd(a, sms);
   if (a.workspace == nullptr || a.workspace_bytes < plan.bytes) return NB_ATTN_ERR_WORKSPACE;
   char* ws = static_cast<char*>(a.workspace);
-  const nb_matrix da{ws + plan.da, s.hidden}, db{ws + plan.db, s.hidden};
-  const nb_matrix h = s.checkpoint == NB_CHECKPOINT_8BIT ? nb_matrix{ws + plan.h, s.hidden} : a.h;
+  const int64_t stride = padded(s.hidden);
+  const nb_matrix da{ws + plan.da, stride}, db{ws + plan.db, stride};
+  const nb_matrix h = s.checkpoint == NB_CHECKPOINT_8BIT ? nb_matrix{ws + plan.h, stride} : a.h;
   const int row_tiles = div_up(s.tokens, kGemmRows);
 
   // dh = dy Wd with the activation's backward behind it. (Needed for every gradient but those of Wd, in 16 bits, and bd.)
@@ -569,10 +575,7 @@ extern "C" int nb_gated_mlp_bwd(const nb_gated_mlp_bwd_args* args, void* stream)
     p.b_mn = 1;
     NB_TRY(map_k_major(&p.a[0], a.dy, s.tokens, s.dim, kGemmRows));
     NB_TRY(map_mn_major(&p.b[0], a.w_down, s.dim, s.hidden));
-    NB_TRY(host_matrix_map(&p.c, da.ptr, s.tokens, s.hidden, da.stride, 32, kGroup));
-    NB_TRY(host_matrix_map(&g.db, db.ptr, s.tokens, s.hidden, db.stride, 32, kGroup));
-    if (s.checkpoint == NB_CHECKPOINT_8BIT)
-      NB_TRY(host_matrix_map(&g.h, h.ptr, s.tokens, s.hidden, h.stride, 32, kGroup));
+    g.da = static_cast<bf16*>(da.ptr), g.db = static_cast<bf16*>(db.ptr), g.h = static_cast<bf16*>(h.ptr), g.stride = da.stride;
     g.codes = static_cast<uint8_t*>(const_cast<void*>(a.checkpoint));
     g.groups = div_up(s.hidden, kGroup), g.hidden = s.hidden;
     if (a.d_b_gate != nullptr || a.d_b_up != nullptr) g.col_sums = reinterpret_cast<float*>(ws + plan.col_sums);

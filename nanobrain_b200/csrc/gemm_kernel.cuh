@@ -22,7 +22,6 @@
 namespace nb {
 
 constexpr int kGemmRows = 128, kGemmDepth = 64, kGemmMaxCols = 256;
-constexpr int kGemmThreads = 384;
 constexpr int kGemmBytesA = kGemmRows * kGemmDepth * 2, kGemmBytesB = kGemmMaxCols * kGemmDepth * 2;
 constexpr int kGroup = 32;  // features of a token that share a scale in the checkpoint
 
@@ -38,14 +37,15 @@ struct CodeBlock {
   static constexpr int kBytes = kBits ? kScales + 128 : 0;
 };
 
-// Shared memory: stages, then a part for every epilogue warp (what it hands to TMA, and code blocks), then barriers.
-constexpr int kEpilogueWarps = 8;
+// Shared memory: stages, then a part for every epilogue warp (a box for TMA's store, or code blocks), then barriers.
 template <int kKind, int kBits, int kCtas>
-struct GemmSmem {
+struct GemmLayout {
+  static constexpr int kTeams = kKind == kGemmPlain ? 2 : 3;  // of four warps, for the 128 rows of a tile
+  static constexpr int kEpilogueWarps = 4 * kTeams;
+  static constexpr int kThreads = 128 + 32 * kEpilogueWarps;
   static constexpr int kStageBytes = kGemmBytesA + kGemmBytesB / kCtas;
-  static constexpr int kTiles = kKind == kGemmPlain ? 4096 : kKind == kGemmGate ? 2048 : (kBits == 8 ? 3 : 2) * 2048;
-  static constexpr int kCodes = kKind == kGemmDact ? 2 : 1;  // code blocks
-  static constexpr int kWarpBytes = (kTiles + kCodes * CodeBlock<kBits>::kBytes + 1023) / 1024 * 1024;
+  static constexpr int kSlots = kKind != kGemmDact ? 0 : kBits == 8 ? 2 : 1;  // code blocks under way
+  static constexpr int kWarpBytes = kKind == kGemmPlain ? 4096 : kSlots * CodeBlock<kBits>::kBytes;
   static constexpr int kMost = 232448 - 1024 - 512 - kEpilogueWarps * kWarpBytes;
   static constexpr int kStages = kMost / kStageBytes < 6 ? kMost / kStageBytes : 6;
   static constexpr int kWarps = kStages * kStageBytes;
@@ -90,13 +90,13 @@ struct GemmParams {
   GemmProblem p[kProblems];
   GemmDeal deal;
   int32_t* status;
-  // the gate's and its backward's: p[0].c = h or da, then
-  CUtensorMap db, h;
+  // the gate's and its backward's
+  __nv_bfloat16 *da, *db, *h;  // rows of `stride` values, at 32 bytes
+  int64_t stride;
   const __nv_bfloat16* bias_up;
   uint8_t* codes;     // checkpoint: [row tile][group][warp] code blocks
   float* col_sums;    // backward: [row tile][warp][2 x hidden] sums of da and db over 32 rows, or NULL
   int32_t groups, hidden;
-  int32_t write_h;
 };
 
 struct GemmUnit {
@@ -137,40 +137,65 @@ constexpr int kActSilu = 0, kActGelu = 1;
 //   gelu: a Phi(a); slope Phi + a phi. Phi by Abramowitz and Stegun 7.1.26: with z = |a| / sqrt 2, t = 1 / (1 + 0.3275911 z),
 //   erfc(z) = t (a1 + t (a2 + t (a3 + t (a4 + t a5)))) e^-z^2, off by at most 1.5e-7; its exponential is phi's as well.
 // Both take one exponential and one reciprocal. A large negative a must give 0 and not 0 x inf: e^-a overflows to inf,
-// whose reciprocal is 0.
+// whose reciprocal is 0. The epilogues are bound by their instructions, so two values go through one packed instruction.
+__device__ __forceinline__ float fast_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint64_t both(float v) { return pack_f32x2(v, v); }
+__device__ __forceinline__ uint64_t exp2_of(uint64_t v) {
+  float x, y;
+  unpack_f32x2(v, x, y);
+  return pack_f32x2(fast_exp2(x), fast_exp2(y));
+}
+__device__ __forceinline__ uint64_t rcp_of(uint64_t v) {
+  float x, y;
+  unpack_f32x2(v, x, y);
+  return pack_f32x2(fast_rcp(x), fast_rcp(y));
+}
+// 1 / (1 + e^-a), or Phi(a) with e = e^(-a^2 / 2).
+__device__ __forceinline__ uint64_t sigmoid_of(uint64_t a) {
+  return rcp_of(add_f32x2(exp2_of(mul_f32x2(a, both(-1.4426950408889634f))), both(1.f)));
+}
+__device__ __forceinline__ uint64_t phi_of(uint64_t a, uint64_t& e) {
+  const uint64_t mag = a & 0x7FFFFFFF7FFFFFFFull;
+  const uint64_t t = rcp_of(fma_f32x2(mag, both(0.3275911f * 0.70710678118654752f), both(1.f)));
+  e = exp2_of(mul_f32x2(mul_f32x2(a, both(-0.72134752044448170f)), a));
+  uint64_t q = fma_f32x2(t, both(1.061405429f), both(-1.453152027f));
+  q = fma_f32x2(t, q, both(1.421413741f));
+  q = fma_f32x2(t, q, both(-0.284496736f));
+  q = fma_f32x2(t, q, both(0.254829592f));
+  q = mul_f32x2(mul_f32x2(t, both(0.5f)), mul_f32x2(q, e));  // Phi(-|a|)
+  float x, y, qx, qy;
+  unpack_f32x2(a, x, y);
+  unpack_f32x2(q, qx, qy);
+  return pack_f32x2(x < 0.f ? qx : 1.f - qx, y < 0.f ? qy : 1.f - qy);
+}
 template <int kAct>
-__device__ __forceinline__ float gate_of(float a) {
+__device__ __forceinline__ uint64_t gate_of(uint64_t a) {
+  uint64_t e;
+  if constexpr (kAct == kActSilu) return mul_f32x2(a, sigmoid_of(a));
+  else return mul_f32x2(a, phi_of(a, e));
+}
+template <int kAct>
+__device__ __forceinline__ void gate_and_slope(uint64_t a, uint64_t& gate, uint64_t& slope) {
   if constexpr (kAct == kActSilu) {
-    return __fdividef(1.f, 1.f + fast_exp2(a * -1.4426950408889634f)) * a;
+    const uint64_t s = sigmoid_of(a);
+    gate = mul_f32x2(a, s);
+    slope = fma_f32x2(gate, fma_f32x2(s, both(-1.f), both(1.f)), s);
   } else {
-    const float z = fabsf(a) * 0.70710678118654752f;
-    const float t = __fdividef(1.f, fmaf(0.3275911f, z, 1.f));
-    const float e = fast_exp2(a * a * -0.72134752044448170f);
-    float q = fmaf(t, 1.061405429f, -1.453152027f);
-    q = fmaf(t, q, 1.421413741f);
-    q = fmaf(t, q, -0.284496736f);
-    q = fmaf(t, q, 0.254829592f) * t * 0.5f * e;  // Phi(-|a|)
-    return a * (a < 0.f ? q : 1.f - q);
+    uint64_t e;
+    const uint64_t phi = phi_of(a, e);
+    gate = mul_f32x2(a, phi);
+    slope = fma_f32x2(mul_f32x2(a, both(0.39894228040143268f)), e, phi);
   }
 }
 template <int kAct>
-__device__ __forceinline__ void gate_and_slope(float a, float& gate, float& slope) {
-  if constexpr (kAct == kActSilu) {
-    const float s = __fdividef(1.f, 1.f + fast_exp2(a * -1.4426950408889634f));
-    gate = a * s;
-    slope = fmaf(gate, 1.f - s, s);
-  } else {
-    const float z = fabsf(a) * 0.70710678118654752f;
-    const float t = __fdividef(1.f, fmaf(0.3275911f, z, 1.f));
-    const float e = fast_exp2(a * a * -0.72134752044448170f);
-    float q = fmaf(t, 1.061405429f, -1.453152027f);
-    q = fmaf(t, q, 1.421413741f);
-    q = fmaf(t, q, -0.284496736f);
-    q = fmaf(t, q, 0.254829592f) * t * 0.5f * e;
-    const float phi = a < 0.f ? q : 1.f - q;
-    gate = a * phi;
-    slope = fmaf(a * 0.39894228040143268f, e, phi);
-  }
+__device__ __forceinline__ float gate_of(float a) {
+  float x, y;
+  unpack_f32x2(gate_of<kAct>(both(a)), x, y);
+  return x;
 }
 
 // ---- the checkpoint ------------------------------------------------------------------------
@@ -178,11 +203,18 @@ __device__ __forceinline__ void gate_and_slope(float a, float& gate, float& slop
 // every value within 2^-29 of it keeps 11 bits (bf16 would keep 8 and cost the gradients a rounding as large as that
 // of their own operands). 8 bits: round(v / s), s = max |v| / 127 rounded up to bf16. A group with a value that is not
 // finite is NaN as a whole in 8 bits; in 16 bits its scale is 1.
+// (four chains of maxima)
 __device__ __forceinline__ float abs_max32(const float (&v)[32]) {
-  float m = 0.f;
+  float m[4];
 #pragma unroll
-  for (int i = 0; i < 32; i += 2) m = max3_nan(m, fabsf(v[i]), fabsf(v[i + 1]));
-  return m;
+  for (int i = 0; i < 4; ++i) m[i] = max3_nan(fabsf(v[i]), fabsf(v[i + 4]), fabsf(v[i + 8]));
+#pragma unroll
+  for (int j = 12; j < 28; j += 8)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m[i] = max3_nan(m[i], fabsf(v[j + i]), fabsf(v[j + 4 + i]));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m[i] = max3_nan(m[i], fabsf(v[28 + i]), 0.f);
+  return max3_nan(max3_nan(m[0], m[1], m[2]), m[3], 0.f);
 }
 
 // Returns the scale as the upper half of its fp32 bits.
@@ -192,10 +224,12 @@ __device__ __forceinline__ uint32_t encode(const float (&v)[32], uint32_t (&w)[C
   if constexpr (kBits == 16) {
     uint32_t e = __float_as_uint(m) >> 23;
     e = e == 255u ? 141u : max(e, 15u);
-    const float inv = __uint_as_float((268u - e) << 23);
+    const uint64_t inv = both(__uint_as_float((268u - e) << 23));
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const __half2 h = __floats2half2_rn(v[2 * i] * inv, v[2 * i + 1] * inv);
+      float x, y;
+      unpack_f32x2(mul_f32x2(pack_f32x2(v[2 * i], v[2 * i + 1]), inv), x, y);
+      const __half2 h = __floats2half2_rn(x, y);
       w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
     return (e - 14u) << 7;
@@ -209,30 +243,36 @@ __device__ __forceinline__ uint32_t encode(const float (&v)[32], uint32_t (&w)[C
     for (int i = 0; i < 8; ++i) {
       uint32_t b[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) b[k] = __float_as_uint(fmaf(v[4 * i + k], inv, 12582912.f));
+      for (int k = 0; k < 4; k += 2) {
+        float x, y;
+        unpack_f32x2(fma_f32x2(pack_f32x2(v[4 * i + k], v[4 * i + k + 1]), both(inv), both(12582912.f)), x, y);
+        b[k] = __float_as_uint(x), b[k + 1] = __float_as_uint(y);
+      }
       w[i] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
     }
     return s;
   }
 }
 
-// Value i of the 32 (i known at compile time).
-template <int kBits>
-__device__ __forceinline__ float decode(const uint32_t (&w)[CodeBlock<kBits>::kWords], int i, float scale) {
+// Values 2 i and 2 i + 1 of a lane's (i known at compile time).
+template <int kBits, int kWords>
+__device__ __forceinline__ uint64_t decode(const uint32_t (&w)[kWords], int i, uint64_t scale) {
   if constexpr (kBits == 16) {
-    const __half2 h = *reinterpret_cast<const __half2*>(&w[i >> 1]);
-    return ((i & 1) ? __high2float(h) : __low2float(h)) * scale;
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    return mul_f32x2(pack_f32x2(f.x, f.y), scale);
   } else {
-    // The code with its sign bit turned, in the low byte of 2^23: 2^23 + code + 128.
-    const uint32_t u = __byte_perm(w[i >> 2] ^ 0x80808080u, 0x4B000000u, 0x7440 | (i & 3));
-    return (__uint_as_float(u) - 8388736.f) * scale;
+    // The codes with their sign bits turned, in the low byte of 2^23: 2^23 + code + 128.
+    const uint32_t u = w[i >> 1] ^ 0x80808080u;
+    const float x = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 | (2 * (i & 1)))),
+                y = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 | (2 * (i & 1) + 1)));
+    return mul_f32x2(add_f32x2(pack_f32x2(x, y), both(-8388736.f)), scale);
   }
 }
 
-// Sum of each of 32 values over the warp's lanes; lane l receives that of value l.
-__device__ __forceinline__ float column_sums(float (&v)[32], int lane) {
+// Sum of each of 16 values over the warp's lanes; lane l receives that of value l % 16.
+__device__ __forceinline__ float column_sums(float (&v)[16], int lane) {
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
+  for (int off = 8; off > 0; off >>= 1) {
     const bool up = (lane & off) != 0;
 #pragma unroll
     for (int i = 0; i < off; ++i) {
@@ -240,7 +280,7 @@ __device__ __forceinline__ float column_sums(float (&v)[32], int lane) {
       v[i] = keep + __shfl_xor_sync(0xffffffffu, send, off);
     }
   }
-  return v[0];
+  return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 16);
 }
 
 __device__ __forceinline__ void add_bias32(float (&v)[32], const __nv_bfloat16* bias, int col, int n) {
@@ -266,20 +306,19 @@ __device__ __forceinline__ void tmem_ld32f(uint32_t taddr, float (&v)[32]) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// 32 values of a row of a box that TMA stores, 64 columns (`half` of it) or 32 wide: the chunks of 16 bytes where its
-// swizzle over 128 or 64 bytes expects them.
+// 32 values of a row of a box that TMA stores, 64 columns wide (`half` of it): the chunks of 16 bytes where its swizzle
+// expects them.
 __device__ __forceinline__ void stage_half_row(uint32_t box, int row, int half, const float (&v)[32]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     st_shared_v4(box + swz128(row, half * 4 + i), pack_bf16(v[8 * i], v[8 * i + 1]), pack_bf16(v[8 * i + 2], v[8 * i + 3]),
                  pack_bf16(v[8 * i + 4], v[8 * i + 5]), pack_bf16(v[8 * i + 6], v[8 * i + 7]));
 }
-__device__ __forceinline__ void stage_row(uint32_t box, int row, const float (&v)[32]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    st_shared_v4(box + row * 64 + ((i ^ ((row >> 1) & 3)) << 4), pack_bf16(v[8 * i], v[8 * i + 1]),
-                 pack_bf16(v[8 * i + 2], v[8 * i + 3]), pack_bf16(v[8 * i + 4], v[8 * i + 5]),
-                 pack_bf16(v[8 * i + 6], v[8 * i + 7]));
+// 16 values to 32 bytes (a whole sector) of a row.
+__device__ __forceinline__ void store_sector(__nv_bfloat16* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
 }
 __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
   uint4 v;
@@ -289,24 +328,25 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
 
 // ---- the kernel ----------------------------------------------------------------------------
 template <int kCtas, int kKind, int kAct, int kBits, int kProblems>
-__global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmParams<kProblems> g) {
-  using L = GemmSmem<kKind, kBits, kCtas>;
+__global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas>::kThreads, 1)
+    gemm_kernel(const __grid_constant__ GemmParams<kProblems> g) {
+  using L = GemmLayout<kKind, kBits, kCtas>;
   constexpr int kStages = L::kStages;
   constexpr bool kPair = kCtas == 2;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t bars = base + L::kBars;
   const uint32_t full = bars, empty = bars + 8 * kStages, acc_full = bars + 16 * kStages, acc_empty = acc_full + 16,
-                 codes_full = acc_empty + 16, tmem_slot = codes_full + 16 * kEpilogueWarps, abort_at = tmem_slot + 4;
+                 codes_full = acc_empty + 16, tmem_slot = codes_full + 16 * L::kEpilogueWarps, abort_at = tmem_slot + 4;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_raw + (abort_at - smem_u32(smem_raw)));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = kPair ? int(cluster_rank()) : 0;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
-    for (int i = 0; i < 2; ++i) mbar_init(acc_full + 8 * i, 1), mbar_init(acc_empty + 8 * i, 8 * kCtas);
+    for (int i = 0; i < 2; ++i) mbar_init(acc_full + 8 * i, 1), mbar_init(acc_empty + 8 * i, L::kEpilogueWarps * kCtas);
     if constexpr (kKind == kGemmDact)
-      for (int i = 0; i < 2 * kEpilogueWarps; ++i) mbar_init(codes_full + 8 * i, 1);
+      for (int i = 0; i < 2 * L::kEpilogueWarps; ++i) mbar_init(codes_full + 8 * i, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -411,44 +451,49 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
       }
     }
   } else if (warp >= 4) {
-    // A warp works by itself on its 32 rows: it takes every other 32 (plain: 64) columns, hands boxes of 32 rows to TMA
-    // and waits for nobody. Its lane is the row. (With boxes of 128 rows, four warps met at two barriers per box, and the
-    // proxy fence waited for the checkpoint's plain stores: together 38 % of the gate epilogue's time.)
+    // A warp works by itself on its 32 rows (its lane is the row) and on every other 64 columns, or on one piece of 32 columns
+    // in three; it waits for no other warp. 12 warps instead of 8 for the epilogues with much to compute: a warp's own latencies
+    // (tensor memory, exponentials, code blocks) left three quarters of the issue slots empty. Their rows go out as whole
+    // sectors from registers. (Boxes for TMA instead cost a proxy fence and shared memory, which is the stages'.)
     const int wg = (warp >> 2) - 1, quarter = warp & 3;
-    const uint32_t box = base + L::kWarps + (warp - 4) * L::kWarpBytes, block = box + L::kTiles;
+    [[maybe_unused]] const uint32_t own = base + L::kWarps + (warp - 4) * L::kWarpBytes;
     const uint32_t lanes = uint32_t(quarter) << 21;
     const uint32_t acc_free = kPair ? map_to_rank(acc_empty, 0) : acc_empty;  // where the MMAs' issuer waits
     constexpr int kB = kBits ? kBits : 16;
     using Block = CodeBlock<kB>;
+    // The first column of this warp's pieces in the CTA's i-th unit: pieces are dealt out across the units.
+    [[maybe_unused]] const auto first_piece = [&](int i, int pieces) {
+      const int at = (wg - i * pieces) % L::kTeams;
+      return (at < 0 ? at + L::kTeams : at) * 32;
+    };
     const auto rows_of = [&](const GemmUnit& u) { return (u.row * kCtas + rank) * kGemmRows; };
     const auto code_block = [&](const GemmUnit& u, int f) {
       return g.codes + ((int64_t(u.row * kCtas + rank) * g.groups + f / kGroup) * 4 + quarter) * Block::kBytes;
     };
 
-    // The backward's code blocks arrive two pieces ahead of their use.
+    // The backward's code blocks are requested as soon as there is room.
     [[maybe_unused]] struct { int i, blk; GemmUnit u; bool live; } ahead{-1, 0, {}, true};
     [[maybe_unused]] uint32_t piece = 0;
     [[maybe_unused]] const uint32_t my_codes = codes_full + 16 * (warp - 4);
     [[maybe_unused]] const auto request = [&](uint32_t slot) {  // the next piece's
       if constexpr (kKind == kGemmDact) {
         const int cols = g.p[0].cols;
-        ahead.blk += 64;
+        ahead.blk += 32 * L::kTeams;
         while (ahead.live && (ahead.i < 0 || ahead.blk >= cols || ahead.u.col * cols + ahead.blk >= g.hidden ||
                               (kPair && rows_of(ahead.u) >= g.p[0].m))) {
           const int id = g.deal.template unit<kCtas>(++ahead.i);
           ahead.live = id >= 0;
           if (ahead.live) ahead.u = gemm_unit(g, id);
-          ahead.blk = wg * 32;
+          ahead.blk = first_piece(ahead.i, cols / 32);
         }
         if (ahead.live && lane == 0) {
           mbar_arrive_expect_tx(my_codes + 8 * slot, Block::kBytes);
-          bulk_load(block + slot * Block::kBytes, code_block(ahead.u, ahead.u.col * cols + ahead.blk), Block::kBytes,
+          bulk_load(own + slot * Block::kBytes, code_block(ahead.u, ahead.u.col * cols + ahead.blk), Block::kBytes,
                     my_codes + 8 * slot);
         }
       }
     };
-    request(0);
-    request(1);
+    for (int i = 0; i < L::kSlots; ++i) request(i);
 
     for (int i = 0;; ++i) {
       const int id = g.deal.template unit<kCtas>(i);
@@ -463,89 +508,102 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         // the pair's second half lies behind the last row
       } else if constexpr (kKind == kGemmGate) {
         const int half = p.cols / 2;
+        __nv_bfloat16* h_row = g.h + int64_t(row + lane) * g.stride;
 #pragma unroll 1
-        for (int blk = wg * 32; blk < half; blk += 64) {
+        for (int blk = first_piece(i, half / 32); blk < half; blk += 32 * L::kTeams) {
           const int f = u.col * half + blk;
           if (f >= g.hidden) break;
+          [[maybe_unused]] uint8_t* block = kBits > 0 ? code_block(u, f) : nullptr;
           float a[32], b[32];
+          [[maybe_unused]] uint32_t w[Block::kWords], scales = 0;
           tmem_ld32f(acc + blk, a);
-          tmem_ld32f(acc + half + blk, b);
           add_bias32(a, p.bias, f, g.hidden);
-          add_bias32(b, g.bias_up, f, g.hidden);
-          if (lane == 0) bulk_wait_group_read0();  // the boxes in front have left
-          __syncwarp();
           if constexpr (kBits > 0) {
-            uint32_t w[Block::kWords];
-            uint32_t scales = encode<kB>(a, w);
+            scales = encode<kB>(a, w);
 #pragma unroll
             for (int c = 0; c < Block::kChunks; ++c)
-              st_shared_v4(block + c * 512 + lane * 16, w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+              *reinterpret_cast<uint4*>(block + c * 512 + lane * 16) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+          }
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) unpack_f32x2(gate_of<kAct>(pack_f32x2(a[k], a[k + 1])), a[k], a[k + 1]);
+          tmem_ld32f(acc + half + blk, b);
+          add_bias32(b, g.bias_up, f, g.hidden);
+          if constexpr (kBits > 0) {
             scales |= encode<kB>(b, w) << 16;
 #pragma unroll
             for (int c = 0; c < Block::kChunks; ++c)
-              st_shared_v4(block + (Block::kChunks + c) * 512 + lane * 16, w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(block + Block::kScales + lane * 4), "r"(scales) : "memory");
+              *reinterpret_cast<uint4*>(block + (Block::kChunks + c) * 512 + lane * 16) =
+                  make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+            *reinterpret_cast<uint32_t*>(block + Block::kScales + lane * 4) = scales;
           }
 #pragma unroll
-          for (int k = 0; k < 32; ++k) a[k] = gate_of<kAct>(a[k]) * b[k];
-          stage_row(box, lane, a);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_2d(&p.c, box, f, row);
-            if constexpr (kBits > 0) bulk_store(code_block(u, f), block, Block::kBytes);
-            bulk_commit_group();
+          for (int q = 0; q < 2; ++q) {
+            uint32_t v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = pack_bf16(a[16 * q + 2 * k] * b[16 * q + 2 * k], a[16 * q + 2 * k + 1] * b[16 * q + 2 * k + 1]);
+            if (row + lane < p.m) store_sector(h_row + f + 16 * q, v);  // (the rows' padding takes what is behind `hidden`)
           }
         }
       } else if constexpr (kKind == kGemmDact) {
+        const int64_t at_row = int64_t(row + lane) * g.stride;
 #pragma unroll 1
-        for (int blk = wg * 32; blk < p.cols; blk += 64) {
+        for (int blk = first_piece(i, p.cols / 32); blk < p.cols; blk += 32 * L::kTeams) {
           const int f = u.col * p.cols + blk;
           if (f >= g.hidden) break;
-          const uint32_t slot = piece & 1, codes = block + slot * Block::kBytes;
-          mbar_wait(my_codes + 8 * slot, (piece >> 1) & 1, abort_flag);
-          uint32_t wa[Block::kWords], wb[Block::kWords], scales;
-#pragma unroll
-          for (int c = 0; c < Block::kChunks; ++c) {
-            const uint4 x = ld_shared_v4(codes + c * 512 + lane * 16),
-                        y = ld_shared_v4(codes + (Block::kChunks + c) * 512 + lane * 16);
-            wa[4 * c] = x.x, wa[4 * c + 1] = x.y, wa[4 * c + 2] = x.z, wa[4 * c + 3] = x.w;
-            wb[4 * c] = y.x, wb[4 * c + 1] = y.y, wb[4 * c + 2] = y.z, wb[4 * c + 3] = y.w;
-          }
+          const uint32_t slot = piece % L::kSlots, codes = own + slot * Block::kBytes;
+          mbar_wait(my_codes + 8 * slot, (piece / L::kSlots) & 1, abort_flag);
+          uint32_t scales;
           asm volatile("ld.shared.b32 %0, [%1];" : "=r"(scales) : "r"(codes + Block::kScales + lane * 4) : "memory");
-          __syncwarp();
-          request(slot);
-          ++piece;
-          const float sa = __uint_as_float(scales << 16), sb = __uint_as_float(scales & 0xFFFF0000u);
-          float d[32], e[32], h[32];
-          tmem_ld32f(acc + blk, d);
+          const uint64_t sa = both(__uint_as_float(scales << 16)), sb = both(__uint_as_float(scales & 0xFFFF0000u));
+          constexpr int kHalf = Block::kChunks / 2;  // chunks of 16 values
 #pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            const float a = decode<kB>(wa, k, sa), b = decode<kB>(wb, k, sb);
-            float gate, slope;
-            gate_and_slope<kAct>(a, gate, slope);
-            e[k] = d[k] * gate;
-            if constexpr (kBits == 8) h[k] = gate * b;
-            d[k] = d[k] * b * slope;
+          for (int q = 0; q < 2; ++q) {
+            uint32_t wa[4 * kHalf], wb[4 * kHalf], r[16];
+            tmem_ld16(acc + blk + 16 * q, r);
+#pragma unroll
+            for (int c = 0; c < kHalf; ++c) {
+              const uint4 x = ld_shared_v4(codes + (q * kHalf + c) * 512 + lane * 16),
+                          y = ld_shared_v4(codes + (Block::kChunks + q * kHalf + c) * 512 + lane * 16);
+              wa[4 * c] = x.x, wa[4 * c + 1] = x.y, wa[4 * c + 2] = x.z, wa[4 * c + 3] = x.w;
+              wb[4 * c] = y.x, wb[4 * c + 1] = y.y, wb[4 * c + 2] = y.z, wb[4 * c + 3] = y.w;
+            }
+            tmem_wait_ld();
+            if (q == 1) {  // the block has been read
+              __syncwarp();
+              request(slot);
+            }
+            float d[16], e[16];
+            uint32_t vd[8], ve[8], vh[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const uint64_t a = decode<kB>(wa, k, sa), b = decode<kB>(wb, k, sb),
+                             dh = pack_f32x2(__uint_as_float(r[2 * k]), __uint_as_float(r[2 * k + 1]));
+              uint64_t gate, slope;
+              gate_and_slope<kAct>(a, gate, slope);
+              unpack_f32x2(mul_f32x2(dh, gate), e[2 * k], e[2 * k + 1]);
+              unpack_f32x2(mul_f32x2(mul_f32x2(dh, b), slope), d[2 * k], d[2 * k + 1]);
+              vd[k] = pack_bf16(d[2 * k], d[2 * k + 1]);
+              ve[k] = pack_bf16(e[2 * k], e[2 * k + 1]);
+              if constexpr (kBits == 8) {
+                float x, y;
+                unpack_f32x2(mul_f32x2(gate, b), x, y);
+                vh[k] = pack_bf16(x, y);
+              }
+            }
+            const int fq = f + 16 * q;
+            if (row + lane < p.m && fq < g.hidden) {
+              store_sector(g.da + at_row + fq, vd);
+              store_sector(g.db + at_row + fq, ve);
+              if constexpr (kBits == 8) store_sector(g.h + at_row + fq, vh);
+            }
+            if (g.col_sums != nullptr) {
+              float* sums = g.col_sums + (int64_t(row0 / kGemmRows) * 4 + quarter) * (2 * int64_t(g.hidden));
+              const float sd = column_sums(d, lane), se = column_sums(e, lane);
+              const int at = fq + (lane & 15);
+              if (at < g.hidden) sums[(lane < 16 ? 0 : g.hidden) + at] = lane < 16 ? sd : se;
+            }
           }
-          if (lane == 0) bulk_wait_group_read0();
-          __syncwarp();
-          stage_row(box, lane, d);
-          stage_row(box + 2048, lane, e);
-          if constexpr (kBits == 8) stage_row(box + 4096, lane, h);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_2d(&p.c, box, f, row);
-            tma_store_2d(&g.db, box + 2048, f, row);
-            if constexpr (kBits == 8) tma_store_2d(&g.h, box + 4096, f, row);
-            bulk_commit_group();
-          }
-          if (g.col_sums != nullptr) {
-            float* sums = g.col_sums + (int64_t(row0 / kGemmRows) * 4 + quarter) * (2 * int64_t(g.hidden));
-            const float sd = column_sums(d, lane), se = column_sums(e, lane);
-            if (f + lane < g.hidden) sums[f + lane] = sd, sums[g.hidden + f + lane] = se;
-          }
+          ++piece;
         }
       } else {
         const int c0 = u.col * p.cols;
@@ -572,11 +630,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
               float v[32];
               tmem_ld32f(acc + blk + q * 32, v);
               add_bias32(v, p.bias, c0 + blk + q * 32, p.n);
-              stage_half_row(box, lane, q, v);
+              stage_half_row(own, lane, q, v);
             }
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) tma_store_2d(&p.c, box, c0 + blk, row), bulk_commit_group();
+            if (lane == 0) tma_store_2d(&p.c, own, c0 + blk, row), bulk_commit_group();
           }
         }
       }
