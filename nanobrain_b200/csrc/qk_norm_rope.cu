@@ -8,9 +8,11 @@
 // backward. A warp takes a token with all its heads, so that the token's 32 angles are computed once, one per lane,
 // and handed around by shuffles. Four lanes share a row of 64 values: lane j of them holds values [8j, 8j+8) and
 // [32+8j, 32+8j+8), which contain both partners of every pair in either order of pairs, so the rotation needs no
-// exchange and every access is 16 bytes. Sums are in fp32; the one rounding is that of the result to bf16.
-// Angles are products and sums in 64 bits, and whole turns are taken off there: position 2^20 at frequency 1 would keep
-// an error of 0.03 in fp32.
+// exchange and every access is 16 bytes. A lane keeps its eight pairs as first and second partners, two pairs to a
+// packed instruction: with one value per instruction the kernels took 35 (forward) and 72 us (backward) on 26253 tokens of
+// 12 + 12 heads, bound by their instructions; now 31 and 53 (161 and 242 MB: 5.2 and 4.6 TB/s). Sums are in fp32; the one
+// rounding is that of the result to bf16. Angles are products and sums in 64 bits, and whole turns are taken off there: position 2^20 at
+// frequency 1 would keep an error of 0.03 in fp32.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -39,26 +41,50 @@ struct Params {
   Side s[2];
   int64_t units, units_q;       // tokens, or tokens of both sides one after the other
   int32_t shared;               // queries and keys of a token are one unit
+  int32_t one_batch;
   int32_t axes, pos_type, interleaved;
   const float* freqs;
   float eps;
   float* partial;               // backward: [blocks][2][64]
 };
 
-__device__ __forceinline__ float2 unpack2(uint32_t v) {
-  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
+using nb::add_f32x2;
+using nb::fma_f32x2;
+using nb::mul_f32x2;
+using nb::pack_f32x2;
+using nb::unpack_f32x2;
+
+__device__ __forceinline__ uint64_t both(float v) { return pack_f32x2(v, v); }
+__device__ __forceinline__ float sum_of(uint64_t v) {
+  float x, y;
+  unpack_f32x2(v, x, y);
+  return x + y;
 }
 
-// cos and sin of the token's angle of pair `lane`.
-__device__ __forceinline__ float2 turn_of(const Params& p, const Side& s, int64_t batch, int64_t token, int lane) {
-  if (p.axes == 0) return make_float2(1.f, 0.f);
+// The warp's number, known to be the same for its lanes: what follows from it can live in uniform registers.
+__device__ __forceinline__ int warp_index() { return __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0); }
+
+// The position coordinates of a token, as they lie in memory.
+struct Position {
+  int64_t at[NB_ROPE_MAX_AXES];
+};
+__device__ __forceinline__ void load_position(const Params& p, const Side& s, int64_t batch, int64_t token, Position& v) {
   const int64_t at = batch * s.ps[0] + token * s.ps[1];
+#pragma unroll
+  for (int a = 0; a < NB_ROPE_MAX_AXES; ++a) {
+    if (a >= p.axes) break;
+    if (p.pos_type == NB_POSITION_I64) v.at[a] = static_cast<const int64_t*>(s.pos)[at + a];
+    else v.at[a] = static_cast<const int32_t*>(s.pos)[at + a];  // (or the bits of a float)
+  }
+}
+// cos and sin of the token's angle of pair `lane`.
+__device__ __forceinline__ float2 turn_of(const Params& p, const Position& v, int lane) {
+  if (p.axes == 0) return make_float2(1.f, 0.f);
   double angle = 0.0;
-  for (int a = 0; a < p.axes; ++a) {
-    double pos;
-    if (p.pos_type == NB_POSITION_I64) pos = double(static_cast<const int64_t*>(s.pos)[at + a]);
-    else if (p.pos_type == NB_POSITION_I32) pos = double(static_cast<const int32_t*>(s.pos)[at + a]);
-    else pos = double(static_cast<const float*>(s.pos)[at + a]);
+#pragma unroll
+  for (int a = 0; a < NB_ROPE_MAX_AXES; ++a) {
+    if (a >= p.axes) break;
+    const double pos = p.pos_type == NB_POSITION_F32 ? double(__int_as_float(int(v.at[a]))) : double(v.at[a]);
     angle = fma(pos, double(p.freqs[a * kPairs + lane]), angle);
   }
   // Whole turns off, in 64 bits; the rest in half turns, which need no reduction.
@@ -68,254 +94,285 @@ __device__ __forceinline__ float2 turn_of(const Params& p, const Side& s, int64_
   return make_float2(cs, sn);
 }
 
-// The eight (cos, sin) that a lane with column block j needs, from the lanes that hold them: those of its values'
-// pairs, 8j + e, or interleaved 4j + e (first eight values) and 16 + 4j + e (the others), e < 4.
-__device__ __forceinline__ void spread(float2 mine, int j, bool interleaved, float (&c)[8], float (&s)[8]) {
+// Pair e (0..7) of a lane with column block j: 8j + e, or interleaved 4j + e of the first eight values and 16 + 4j + e of
+// the others.
+template <bool kInter>
+__device__ __forceinline__ int pair_of(int j, int e) {
+  return kInter ? (e < 4 ? 4 * j + e : 16 + 4 * j + (e - 4)) : 8 * j + e;
+}
+// cos and sin of the lane's pairs, from the lanes that hold them.
+template <bool kInter>
+__device__ __forceinline__ void spread(float2 mine, int j, uint64_t (&c)[4], uint64_t (&s)[4]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int src = interleaved ? (e < 4 ? 4 * j + e : 16 + 4 * j + (e - 4)) : 8 * j + e;
-    c[e] = __shfl_sync(0xffffffffu, mine.x, src);
-    s[e] = __shfl_sync(0xffffffffu, mine.y, src);
+  for (int i = 0; i < 4; ++i) {
+    const int p0 = pair_of<kInter>(j, 2 * i), p1 = pair_of<kInter>(j, 2 * i + 1);
+    c[i] = pack_f32x2(__shfl_sync(0xffffffffu, mine.x, p0), __shfl_sync(0xffffffffu, mine.x, p1));
+    s[i] = pack_f32x2(__shfl_sync(0xffffffffu, mine.y, p0), __shfl_sync(0xffffffffu, mine.y, p1));
   }
 }
 
-// v: a lane's 16 values, first the eight of block j, then those of block 4 + j. Turned by the angles, or back.
-template <bool kBack>
-__device__ __forceinline__ void rotate(float (&v)[16], const float (&c)[8], const float (&s)[8], bool interleaved) {
-  if (interleaved) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float a = v[2 * e], b = v[2 * e + 1], t = kBack ? -s[e] : s[e];
-      v[2 * e] = a * c[e] - b * t;
-      v[2 * e + 1] = b * c[e] + a * t;
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float a = v[e], b = v[8 + e], t = kBack ? -s[e] : s[e];
-      v[e] = a * c[e] - b * t;
-      v[8 + e] = b * c[e] + a * t;
-    }
-  }
-}
-
-__device__ __forceinline__ void to_float(const uint4& lo, const uint4& hi, float (&v)[16]) {
+// A lane's 16 values as the first and second partners of its eight pairs.
+template <bool kInter>
+__device__ __forceinline__ void partners(const uint4& lo, const uint4& hi, uint64_t (&a)[4], uint64_t (&b)[4]) {
   const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 f = unpack2(w[i]);
-    v[2 * i] = f.x, v[2 * i + 1] = f.y;
+  for (int i = 0; i < 4; ++i) {
+    const auto low = [](uint32_t v) { return __uint_as_float(v << 16); };
+    const auto high = [](uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); };
+    if constexpr (kInter) {
+      a[i] = pack_f32x2(low(w[2 * i]), low(w[2 * i + 1]));
+      b[i] = pack_f32x2(high(w[2 * i]), high(w[2 * i + 1]));
+    } else {
+      a[i] = pack_f32x2(low(w[i]), high(w[i]));
+      b[i] = pack_f32x2(low(w[4 + i]), high(w[4 + i]));
+    }
   }
 }
-__device__ __forceinline__ void store16(__nv_bfloat16* p, int j, const float (&v)[16]) {
-  uint4 lo, hi;
-  lo.x = nb::pack_bf16(v[0], v[1]), lo.y = nb::pack_bf16(v[2], v[3]);
-  lo.z = nb::pack_bf16(v[4], v[5]), lo.w = nb::pack_bf16(v[6], v[7]);
-  hi.x = nb::pack_bf16(v[8], v[9]), hi.y = nb::pack_bf16(v[10], v[11]);
-  hi.z = nb::pack_bf16(v[12], v[13]), hi.w = nb::pack_bf16(v[14], v[15]);
-  *reinterpret_cast<uint4*>(p + 8 * j) = lo;
-  *reinterpret_cast<uint4*>(p + 32 + 8 * j) = hi;
+template <bool kInter>
+__device__ __forceinline__ void store16(__nv_bfloat16* p, int j, const uint64_t (&a)[4], const uint64_t (&b)[4]) {
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a0, a1, b0, b1;
+    unpack_f32x2(a[i], a0, a1);
+    unpack_f32x2(b[i], b0, b1);
+    if constexpr (kInter) w[2 * i] = nb::pack_bf16(a0, b0), w[2 * i + 1] = nb::pack_bf16(a1, b1);
+    else w[i] = nb::pack_bf16(a0, a1), w[4 + i] = nb::pack_bf16(b0, b1);
+  }
+  *reinterpret_cast<uint4*>(p + 8 * j) = make_uint4(w[0], w[1], w[2], w[3]);
+  *reinterpret_cast<uint4*>(p + 32 + 8 * j) = make_uint4(w[4], w[5], w[6], w[7]);
+}
+// Where value `a` or `b` of pair e of column block j lies in the row.
+template <bool kInter>
+__device__ __forceinline__ int column_of(int j, int e, bool second) {
+  const int pair = pair_of<kInter>(j, e);
+  return kInter ? 2 * pair + second : pair + 32 * second;
+}
+
+// (a, b) turned by the angles, or back (s negated).
+__device__ __forceinline__ void rotate(uint64_t (&a)[4], uint64_t (&b)[4], const uint64_t (&c)[4], const uint64_t (&s)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint64_t x = a[i], y = b[i], n = s[i] ^ 0x8000000080000000ull;
+    a[i] = fma_f32x2(y, n, mul_f32x2(x, c[i]));
+    b[i] = fma_f32x2(x, s[i], mul_f32x2(y, c[i]));
+  }
 }
 __device__ __forceinline__ float sum4(float v) {
   v += __shfl_xor_sync(0xffffffffu, v, 1);
   return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
-
-// What a unit is: a token of one side, or of both.
-struct Unit {
-  int side, rows;          // the first row's side; rows of the unit
-  int64_t batch, token;
-};
-__device__ __forceinline__ Unit unit_of(const Params& p, int64_t u) {
-  Unit r;
-  r.side = p.shared || u < p.units_q ? 0 : 1;
-  const uint32_t at = uint32_t(r.side ? u - p.units_q : u), len = uint32_t(p.s[r.side].tokens);
-  const uint32_t b = at / len;
-  r.batch = b, r.token = at - b * len;
-  r.rows = p.shared ? p.s[0].heads + p.s[1].heads : p.s[r.side].heads;
-  return r;
+// (mean x^2 + eps)^-1/2 of the row.
+__device__ __forceinline__ float root_of(const uint64_t (&a)[4], const uint64_t (&b)[4], float eps) {
+  uint64_t ss = mul_f32x2(a[0], a[0]);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) ss = fma_f32x2(a[i], a[i], ss);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) ss = fma_f32x2(b[i], b[i], ss);
+  return rsqrtf(sum4(sum_of(ss)) * (1.f / kDim) + eps);
 }
 
-// The weights of both sides in shared memory: [2][64].
+// A warp's way through its units (tokens of one side, or of both) and their groups of eight rows. All of it is the same for
+// the warp's lanes.
+struct Walk {
+  int64_t unit, batch, token;
+  int side, r0, split, rows;  // rows from `split` on are keys
+  bool live;
+};
+__device__ __forceinline__ void enter(const Params& p, Walk& w) {
+  w.live = w.unit < p.units;
+  if (!w.live) return;
+  w.side = p.shared || w.unit < p.units_q ? 0 : 1;
+  const uint32_t at = uint32_t(w.side ? w.unit - p.units_q : w.unit), len = uint32_t(p.s[w.side].tokens);
+  const uint32_t b = p.one_batch ? 0 : at / len;
+  w.batch = b, w.token = at - b * len;
+  w.r0 = 0;
+  w.split = w.side ? 0 : p.s[0].heads;
+  w.rows = w.split + (p.shared || w.side ? p.s[1].heads : 0);
+}
+__device__ __forceinline__ Walk begin(const Params& p, int warp) {
+  Walk w{};
+  w.unit = int64_t(blockIdx.x) * kWarps + warp;
+  enter(p, w);
+  return w;
+}
+__device__ __forceinline__ void advance(const Params& p, Walk& w) {
+  w.r0 += kRowsAtOnce;
+  if (w.r0 < w.rows) return;
+  w.unit += int64_t(gridDim.x) * kWarps;
+  enter(p, w);
+}
+// A lane's row of the group in a tensor with these strides.
+template <typename T>
+__device__ __forceinline__ T* row_of(T* q, const int64_t (&sq)[3], T* k, const int64_t (&sk)[3], const Walk& w, int row) {
+  return row < w.split ? q + w.batch * sq[0] + w.token * sq[1] + row * sq[2]
+                       : k + w.batch * sk[0] + w.token * sk[1] + (row - w.split) * sk[2];
+}
+
+// The weights of both sides in shared memory, as the lanes hold them: [side][j][first, second][8 pairs].
+template <bool kInter>
 __device__ __forceinline__ void load_weights(const Params& p, float* w) {
   if (threadIdx.x < 2 * kDim) {
-    const float* src = p.s[threadIdx.x / kDim].weight;
-    w[threadIdx.x] = src != nullptr ? src[threadIdx.x % kDim] : 1.f;
+    const int side = threadIdx.x / kDim, j = (threadIdx.x >> 4) & 3, second = (threadIdx.x >> 3) & 1, e = threadIdx.x & 7;
+    const float* src = p.s[side].weight;
+    w[threadIdx.x] = src != nullptr ? src[column_of<kInter>(j, e, second)] : 1.f;
   }
   __syncthreads();
 }
-__device__ __forceinline__ void weights_of(const float* w, int side, int j, float (&v)[16]) {
+__device__ __forceinline__ void weights_of(const float* w, int side, int j, uint64_t (&a)[4], uint64_t (&b)[4]) {
+  const float* at = w + side * kDim + j * 16;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float4 f = *reinterpret_cast<const float4*>(w + side * kDim + (i >> 1) * 32 + 8 * j + (i & 1) * 4);
-    v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
+  for (int i = 0; i < 2; ++i) {
+    const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(at + 4 * i), y = *reinterpret_cast<const ulonglong2*>(at + 8 + 4 * i);
+    a[2 * i] = x.x, a[2 * i + 1] = x.y, b[2 * i] = y.x, b[2 * i + 1] = y.y;
   }
 }
 
 // ---- forward -------------------------------------------------------------------------------
-constexpr int kFwdDeep = 3;  // groups of eight rows whose loads are under way together (12 + 12 heads: all of a token)
+// The next group's rows (and the next token's position) are under way while a group is computed.
+constexpr int kFwdBlocks = 4;  // per SM
 
-__global__ void __launch_bounds__(kThreads) qk_fwd_kernel(const __grid_constant__ Params p) {
+template <bool kInter>
+__global__ void __launch_bounds__(kThreads, kFwdBlocks) qk_fwd_kernel(const __grid_constant__ Params p) {
   __shared__ __align__(16) float w_smem[2 * kDim];
   nb::pdl_wait();
   nb::pdl_launch_dependents();
-  load_weights(p, w_smem);
+  load_weights<kInter>(p, w_smem);
   const int lane = threadIdx.x & 31, j = lane & 3, slot = lane >> 2;
-  const int64_t step = int64_t(gridDim.x) * kWarps;
-  for (int64_t u = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5); u < p.units; u += step) {
-    const Unit unit = unit_of(p, u);
-    float c[8], s[8];
-    for (int r0 = 0; r0 < unit.rows; r0 += kFwdDeep * kRowsAtOnce) {
-      uint4 lo[kFwdDeep], hi[kFwdDeep];
-#pragma unroll
-      for (int d = 0; d < kFwdDeep; ++d) {
-        const int row = r0 + d * kRowsAtOnce + slot;
-        if (row < unit.rows) {
-          const int side = p.shared ? row >= p.s[0].heads : unit.side;
-          const Side& sd = p.s[side];
-          const int head = p.shared && side ? row - p.s[0].heads : row;
-          const __nv_bfloat16* x = sd.x + unit.batch * sd.xs[0] + unit.token * sd.xs[1] + head * sd.xs[2];
-          lo[d] = *reinterpret_cast<const uint4*>(x + 8 * j);
-          hi[d] = *reinterpret_cast<const uint4*>(x + 32 + 8 * j);
-        } else {
-          lo[d] = hi[d] = make_uint4(0, 0, 0, 0);
-        }
-      }
-      if (r0 == 0) spread(turn_of(p, p.s[unit.side], unit.batch, unit.token, lane), j, p.interleaved, c, s);
-#pragma unroll
-      for (int d = 0; d < kFwdDeep; ++d) {
-        if (r0 + d * kRowsAtOnce >= unit.rows) break;
-        const int row = r0 + d * kRowsAtOnce + slot;
-        const int side = p.shared ? row >= p.s[0].heads : unit.side;
-        float v[16], w[16];
-        to_float(lo[d], hi[d], v);
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) ss = fmaf(v[i], v[i], ss);
-        const float r = rsqrtf(sum4(ss) * (1.f / kDim) + p.eps);
-        weights_of(w_smem, side, j, w);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] *= r * w[i];
-        rotate<false>(v, c, s, p.interleaved);
-        if (row < unit.rows) {
-          const Side& sd = p.s[side];
-          const int head = p.shared && side ? row - p.s[0].heads : row;
-          store16(sd.y + unit.batch * sd.ys[0] + unit.token * sd.ys[1] + head * sd.ys[2], j, v);
-        }
-      }
+  uint4 lo = {}, hi = {};
+  Position pos;
+  const auto load = [&](const Walk& w) {
+    const int row = w.r0 + slot;
+    if (row < w.rows) {
+      const __nv_bfloat16* x = row_of(p.s[0].x, p.s[0].xs, p.s[1].x, p.s[1].xs, w, row);
+      lo = *reinterpret_cast<const uint4*>(x + 8 * j);
+      hi = *reinterpret_cast<const uint4*>(x + 32 + 8 * j);
     }
+    if (w.r0 == 0) load_position(p, p.s[w.side], w.batch, w.token, pos);
+  };
+  Walk w = begin(p, warp_index());
+  if (w.live) load(w);
+  uint64_t c[4], s[4];
+  while (w.live) {
+    const Walk now = w;
+    uint64_t a[4], b[4], wa[4], wb[4];
+    partners<kInter>(lo, hi, a, b);
+    if (now.r0 == 0) spread<kInter>(turn_of(p, pos, lane), j, c, s);
+    advance(p, w);
+    if (w.live) load(w);
+    const int row = now.r0 + slot, side = row >= now.split;
+    const uint64_t r = both(root_of(a, b, p.eps));
+    weights_of(w_smem, side, j, wa, wb);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = mul_f32x2(mul_f32x2(a[i], r), wa[i]);
+      b[i] = mul_f32x2(mul_f32x2(b[i], r), wb[i]);
+    }
+    rotate(a, b, c, s);
+    if (row < now.rows) store16<kInter>(row_of(p.s[0].y, p.s[0].ys, p.s[1].y, p.s[1].ys, now, row), j, a, b);
   }
 }
 
 // ---- backward ------------------------------------------------------------------------------
-constexpr int kBwdDeep = 2;
+constexpr int kBwdBlocks = 2;  // per SM
 
-__global__ void __launch_bounds__(kThreads, 2) qk_bwd_kernel(const __grid_constant__ Params p) {
+template <bool kInter>
+__global__ void __launch_bounds__(kThreads, kBwdBlocks) qk_bwd_kernel(const __grid_constant__ Params p) {
   __shared__ __align__(16) float w_smem[2 * kDim];
-  __shared__ float dw_smem[kWarps][2 * kDim];
+  // Every lane's sums of dw of both sides. In registers they are 32 of 128, and the rest spills: 180 instead of 165 us on
+  // 32 x 4096 tokens of 8 + 8 heads. (Three blocks of 80 registers spill as well: 217.)
+  __shared__ __align__(16) ulonglong2 dw_smem[kWarps][2][4][32];
+  const int lane = threadIdx.x & 31, warp = warp_index(), j = lane & 3, slot = lane >> 2;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) dw_smem[warp][0][i][lane] = dw_smem[warp][1][i][lane] = make_ulonglong2(0, 0);
   nb::pdl_wait();
   nb::pdl_launch_dependents();
-  load_weights(p, w_smem);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = lane & 3, slot = lane >> 2;
-  float dw[2][16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) dw[0][i] = dw[1][i] = 0.f;
-  const int64_t step = int64_t(gridDim.x) * kWarps;
-  for (int64_t u = int64_t(blockIdx.x) * kWarps + warp; u < p.units; u += step) {
-    const Unit unit = unit_of(p, u);
-    float c[8], s[8];
-    for (int r0 = 0; r0 < unit.rows; r0 += kBwdDeep * kRowsAtOnce) {
-      uint4 lo[kBwdDeep], hi[kBwdDeep], glo[kBwdDeep], ghi[kBwdDeep];
-#pragma unroll
-      for (int d = 0; d < kBwdDeep; ++d) {
-        const int row = r0 + d * kRowsAtOnce + slot;
-        if (row < unit.rows) {
-          const int side = p.shared ? row >= p.s[0].heads : unit.side;
-          const Side& sd = p.s[side];
-          const int head = p.shared && side ? row - p.s[0].heads : row;
-          const __nv_bfloat16* x = sd.x + unit.batch * sd.xs[0] + unit.token * sd.xs[1] + head * sd.xs[2];
-          const __nv_bfloat16* g = sd.dy + unit.batch * sd.gs[0] + unit.token * sd.gs[1] + head * sd.gs[2];
-          lo[d] = *reinterpret_cast<const uint4*>(x + 8 * j);
-          hi[d] = *reinterpret_cast<const uint4*>(x + 32 + 8 * j);
-          glo[d] = *reinterpret_cast<const uint4*>(g + 8 * j);
-          ghi[d] = *reinterpret_cast<const uint4*>(g + 32 + 8 * j);
-        } else {
-          lo[d] = hi[d] = glo[d] = ghi[d] = make_uint4(0, 0, 0, 0);
-        }
-      }
-      if (r0 == 0) spread(turn_of(p, p.s[unit.side], unit.batch, unit.token, lane), j, p.interleaved, c, s);
-#pragma unroll
-      for (int d = 0; d < kBwdDeep; ++d) {
-        if (r0 + d * kRowsAtOnce >= unit.rows) break;
-        const int row = r0 + d * kRowsAtOnce + slot;
-        const int side = p.shared ? row >= p.s[0].heads : unit.side;
-        float v[16], g[16], w[16];
-        to_float(lo[d], hi[d], v);
-        to_float(glo[d], ghi[d], g);
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) ss = fmaf(v[i], v[i], ss);
-        const float r = rsqrtf(sum4(ss) * (1.f / kDim) + p.eps);
-        rotate<true>(g, c, s, p.interleaved);  // dn
-        weights_of(w_smem, side, j, w);
-        float gx = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          v[i] *= r;  // x r
-          const float t = g[i] * v[i];
-          if (row < unit.rows) {
-            if (side) dw[1][i] += t;
-            else dw[0][i] += t;
-          }
-          gx = fmaf(t, w[i], gx);
-        }
-        const float mean = sum4(gx) * (1.f / kDim);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) g[i] = r * (g[i] * w[i] - v[i] * mean);
-        if (row < unit.rows) {
-          const Side& sd = p.s[side];
-          const int head = p.shared && side ? row - p.s[0].heads : row;
-          store16(sd.y + unit.batch * sd.ys[0] + unit.token * sd.ys[1] + head * sd.ys[2], j, g);
-        }
-      }
+  load_weights<kInter>(p, w_smem);
+  uint4 lo = {}, hi = {}, glo = {}, ghi = {};
+  Position pos;
+  const auto load = [&](const Walk& w) {
+    const int row = w.r0 + slot;
+    if (row < w.rows) {
+      const __nv_bfloat16* x = row_of(p.s[0].x, p.s[0].xs, p.s[1].x, p.s[1].xs, w, row);
+      const __nv_bfloat16* g = row_of(p.s[0].dy, p.s[0].gs, p.s[1].dy, p.s[1].gs, w, row);
+      lo = *reinterpret_cast<const uint4*>(x + 8 * j);
+      hi = *reinterpret_cast<const uint4*>(x + 32 + 8 * j);
+      glo = *reinterpret_cast<const uint4*>(g + 8 * j);
+      ghi = *reinterpret_cast<const uint4*>(g + 32 + 8 * j);
     }
+    if (w.r0 == 0) load_position(p, p.s[w.side], w.batch, w.token, pos);
+  };
+  Walk w = begin(p, warp);
+  if (w.live) load(w);
+  uint64_t c[4], s[4];
+  while (w.live) {
+    const Walk now = w;
+    uint64_t a[4], b[4], ga[4], gb[4], wa[4], wb[4];
+    partners<kInter>(lo, hi, a, b);
+    partners<kInter>(glo, ghi, ga, gb);
+    if (now.r0 == 0) {
+      float2 turn = turn_of(p, pos, lane);
+      turn.y = -turn.y;
+      spread<kInter>(turn, j, c, s);
+    }
+    advance(p, w);
+    if (w.live) load(w);
+    const int row = now.r0 + slot, side = row >= now.split;
+    const uint64_t r = both(root_of(a, b, p.eps));
+    rotate(ga, gb, c, s);  // dn
+    weights_of(w_smem, side, j, wa, wb);
+    uint64_t gx = 0;
+    ulonglong2* dw = &dw_smem[warp][side][0][lane];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = mul_f32x2(a[i], r), b[i] = mul_f32x2(b[i], r);  // x r
+      const uint64_t ta = mul_f32x2(ga[i], a[i]), tb = mul_f32x2(gb[i], b[i]);
+      if (row < now.rows) {
+        const ulonglong2 sum = dw[i * 32];
+        dw[i * 32] = make_ulonglong2(add_f32x2(sum.x, ta), add_f32x2(sum.y, tb));
+      }
+      gx = fma_f32x2(ta, wa[i], gx);
+      gx = fma_f32x2(tb, wb[i], gx);
+    }
+    const uint64_t mean = both(sum4(sum_of(gx)) * (-1.f / kDim));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ga[i] = mul_f32x2(r, fma_f32x2(a[i], mean, mul_f32x2(ga[i], wa[i])));
+      gb[i] = mul_f32x2(r, fma_f32x2(b[i], mean, mul_f32x2(gb[i], wb[i])));
+    }
+    if (row < now.rows) store16<kInter>(row_of(p.s[0].y, p.s[0].ys, p.s[1].y, p.s[1].ys, now, row), j, ga, gb);
   }
-  // The block's sums of dw: over the eight rows of a warp, then over its warps in order.
-#pragma unroll
-  for (int side = 0; side < 2; ++side)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float v = dw[side][i];
-      v += __shfl_xor_sync(0xffffffffu, v, 4);
-      v += __shfl_xor_sync(0xffffffffu, v, 8);
-      v += __shfl_xor_sync(0xffffffffu, v, 16);
-      if (slot == 0) dw_smem[warp][side * kDim + (i >> 3) * 32 + 8 * j + (i & 7)] = v;
-    }
+  // The block's sums of dw, a column per thread: over its warps and their eight rows, in order.
   __syncthreads();
   if (threadIdx.x < 2 * kDim) {
+    const int sd = threadIdx.x / kDim, cj = (threadIdx.x >> 4) & 3, second = (threadIdx.x >> 3) & 1, e = threadIdx.x & 7;
     float v = 0.f;
+    for (int k = 0; k < kWarps; ++k)
 #pragma unroll
-    for (int k = 0; k < kWarps; ++k) v += dw_smem[k][threadIdx.x];
-    p.partial[int64_t(blockIdx.x) * 2 * kDim + threadIdx.x] = v;
+      for (int l = 0; l < 8; ++l)
+        v += reinterpret_cast<const float*>(&dw_smem[k][sd][e >> 1][4 * l + cj])[2 * second + (e & 1)];
+    p.partial[int64_t(blockIdx.x) * 2 * kDim + sd * kDim + column_of<kInter>(cj, e, second)] = v;
   }
 }
 
-// dw of both sides from the blocks' sums, always in the same order: 8 threads a column.
+// dw of both sides from the blocks' sums, always in the same order: a block takes 16 columns, 64 threads a column (one
+// block for all of them waited 7 us for its loads).
+constexpr int kDwColumns = 16;
 __global__ void __launch_bounds__(1024) qk_dw_kernel(const float* partial, int blocks, float* dwq, float* dwk) {
-  __shared__ float part[8][2 * kDim];
+  __shared__ float part[64][kDwColumns + 1];
   nb::pdl_wait();
   nb::pdl_launch_dependents();
-  const int col = threadIdx.x & 127, lane = threadIdx.x >> 7;
+  const int c = threadIdx.x & (kDwColumns - 1), lane = threadIdx.x / kDwColumns, col = blockIdx.x * kDwColumns + c;
   float v = 0.f;
 #pragma unroll 8
-  for (int b = lane; b < blocks; b += 8) v += partial[b * 2 * kDim + col];
-  part[lane][col] = v;
+  for (int b = lane; b < blocks; b += 64) v += partial[b * 2 * kDim + col];
+  part[lane][c] = v;
   __syncthreads();
-  if (threadIdx.x < 2 * kDim) {
+  if (threadIdx.x < kDwColumns) {
     v = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v += part[k][threadIdx.x];
-    (threadIdx.x < kDim ? dwq : dwk)[threadIdx.x % kDim] = v;
+    for (int k = 0; k < 64; ++k) v += part[k][c];
+    (col < kDim ? dwq : dwk)[col % kDim] = v;
   }
 }
 
@@ -380,6 +437,15 @@ int make_params(const nb_qk_norm_rope_args* a, bool bwd, Params* p) {
               (a->axes == 0 || (q.pos == k.pos && q.ps[0] == k.ps[0] && q.ps[1] == k.ps[1]));
   p->units_q = int64_t(a->batch) * q.tokens;
   p->units = p->units_q + (p->shared ? 0 : int64_t(a->batch) * k.tokens);
+  // Batches that follow on one another in every tensor are one long batch: no division per token.
+  p->one_batch = a->batch == 1;
+  const auto follows = [](const int64_t* s, int64_t tokens) { return s[0] == tokens * s[1]; };
+  if (!p->one_batch) {
+    p->one_batch = true;
+    for (const Side& s : p->s)
+      p->one_batch = p->one_batch && follows(s.xs, s.tokens) && follows(s.ys, s.tokens) && (!bwd || follows(s.gs, s.tokens)) &&
+                     (a->axes == 0 || follows(s.ps, s.tokens));
+  }
   p->axes = a->axes, p->pos_type = a->position_type, p->interleaved = a->interleaved != 0;
   p->freqs = a->freqs, p->eps = a->eps;
   return NB_ATTN_OK;
@@ -393,8 +459,9 @@ extern "C" int nb_qk_norm_rope_fwd(const nb_qk_norm_rope_args* args, void* strea
   int sms = 0;
   if (int rc = nb::host_prepare(&sms)) return rc;
   if (p.units == 0) return NB_ATTN_OK;
-  const int64_t blocks = (p.units + kWarps - 1) / kWarps, most = int64_t(sms) * 3;
-  return launch(qk_fwd_kernel, unsigned(blocks < most ? blocks : most), kThreads, stream, p);
+  const int64_t blocks = (p.units + kWarps - 1) / kWarps, most = int64_t(sms) * kFwdBlocks;
+  return launch(p.interleaved ? qk_fwd_kernel<true> : qk_fwd_kernel<false>, unsigned(blocks < most ? blocks : most), kThreads,
+                stream, p);
 }
 
 extern "C" size_t nb_qk_norm_rope_bwd_workspace_bytes(void) { return size_t(kBwdBlocksMax) * 2 * kDim * sizeof(float); }
@@ -409,10 +476,11 @@ extern "C" int nb_qk_norm_rope_bwd(const nb_qk_norm_rope_args* args, void* strea
   if (int rc = nb::host_prepare(&sms)) return rc;
   p.partial = static_cast<float*>(args->workspace);
   int64_t blocks = (p.units + kWarps - 1) / kWarps;
-  const int64_t most = int64_t(sms) * 2 < kBwdBlocksMax ? int64_t(sms) * 2 : kBwdBlocksMax;
+  const int64_t most = int64_t(sms) * kBwdBlocks < kBwdBlocksMax ? int64_t(sms) * kBwdBlocks : kBwdBlocksMax;
   if (blocks > most) blocks = most;
   if (blocks > 0)
-    if (int rc = launch(qk_bwd_kernel, unsigned(blocks), kThreads, stream, p)) return rc;
-  return launch(qk_dw_kernel, 1u, 1024u, stream, static_cast<const float*>(p.partial), int(blocks), args->q.d_weight,
+    if (int rc = launch(p.interleaved ? qk_bwd_kernel<true> : qk_bwd_kernel<false>, unsigned(blocks), kThreads, stream, p))
+      return rc;
+  return launch(qk_dw_kernel, unsigned(2 * kDim / kDwColumns), 1024u, stream, static_cast<const float*>(p.partial), int(blocks), args->q.d_weight,
                 args->k.d_weight);
 }
