@@ -94,6 +94,10 @@ class ViTMAE3D(nn.Module):
         mlp_ratio: float = 4,
         class_tokens: int = 1,
         drop_path_rate: float = 0.0,
+        qk_norm: bool = False,
+        rope: bool = False,
+        mlp: str = "gelu",
+        mlp_checkpoint: str = "16bit",
     ) -> None:
         super().__init__()
         self.grid_size = tuple(grid_size)
@@ -104,13 +108,16 @@ class ViTMAE3D(nn.Module):
         patch_dim = patch_size ** 3
         self.register_buffer("coord_grid", make_coord_grid(grid_size, patch_size), persistent=False)
 
+        # What the reference's blocks do not have (off by default): see modules.Attention and modules.GatedMlp.
+        self.rope = rope
+        more = dict(qk_norm=qk_norm, rope_grid=patch_grid if rope else None, mlp=mlp, mlp_checkpoint=mlp_checkpoint)
         self.patch_embed = nn.Linear(patch_dim, embed_dim)
         self.pos_embed = SeparablePosEmbed3D(patch_grid, embed_dim)
         self.cls_token = nn.Parameter(torch.empty(1, class_tokens, embed_dim)) if class_tokens else None
         dpr = [x.item() for x in torch.linspace(0, drop_path_rate, depth)]
         self.blocks = nn.ModuleList([
             Block(dim=embed_dim, num_heads=num_heads, qkv_bias=qkv_bias, proj_bias=proj_bias, mlp_ratio=mlp_ratio,
-                  drop_path=dpr[i])
+                  drop_path=dpr[i], **more)
             for i in range(depth)
         ])
         self.norm = LayerNorm(embed_dim)
@@ -120,7 +127,7 @@ class ViTMAE3D(nn.Module):
         self.mask_token = nn.Parameter(torch.empty(1, 1, decoder_embed_dim))
         self.decoder_blocks = nn.ModuleList([
             Block(dim=decoder_embed_dim, num_heads=decoder_num_heads, qkv_bias=qkv_bias, proj_bias=proj_bias,
-                  mlp_ratio=mlp_ratio)
+                  mlp_ratio=mlp_ratio, **more)
             for _ in range(decoder_depth)
         ])
         self.decoder_norm = LayerNorm(decoder_embed_dim)
@@ -134,6 +141,14 @@ class ViTMAE3D(nn.Module):
         nn.init.normal_(self.mask_token, std=0.02)
         self.decoder_head.weight.data.mul_(0.0)
 
+    def _rotation(self, *coords: Tensor) -> dict:
+        """The blocks' ``coord`` argument where they rotate: coordinates of a dense sequence's tokens behind its class
+        tokens, which stand at the origin."""
+        if not self.rope:
+            return {}
+        b = coords[0].shape[0]
+        return {"coord": torch.cat([coords[0].new_zeros(b, self.class_tokens, coords[0].shape[2]), *coords], dim=1)}
+
     # ------------------------------------------------------------------ dense (reference) path
     def forward_encoder(self, patches: Tensor, coord: Tensor) -> Tensor:
         """``[B, N, P]`` patches + ``[B, N, 3]`` coordinates -> ``[B, R+N, D]`` (``model.py:124-141``)."""
@@ -141,19 +156,24 @@ class ViTMAE3D(nn.Module):
         x = self.pos_embed(self.patch_embed(patches), coord)
         if self.class_tokens:
             x = torch.cat([self.cls_token.expand(b, -1, -1), x], dim=1)
+        rotation = self._rotation(coord)
         for block in self.blocks:
-            x = block(x)
+            x = block(x, **rotation)
         return self.norm(x)
 
-    def forward_decoder(self, embeds: Tensor, target_coord: Tensor) -> Tensor:
+    def forward_decoder(self, embeds: Tensor, target_coord: Tensor, coord: Optional[Tensor] = None) -> Tensor:
         """``[B, R+N, D]`` encoder tokens + ``[B, M, 3]`` target coordinates -> ``[B, M, P]``
-        predicted patches (``model.py:143-165``): dense attention over all ``R+N+M`` tokens."""
+        predicted patches (``model.py:143-165``): dense attention over all ``R+N+M`` tokens. ``coord``: ``[B, N, 3]``
+        coordinates of the encoder tokens, for a model that rotates queries and keys."""
+        if self.rope and coord is None:
+            raise ValueError("coord is required: this model rotates queries and keys by their tokens' coordinates")
         b, m = embeds.shape[0], target_coord.shape[1]
         embeds = self.decoder_proj(embeds)
         mask_tokens = self.decoder_pos_embed(self.mask_token.expand(b, m, -1), target_coord)
         x = torch.cat([embeds, mask_tokens], dim=1)
+        rotation = self._rotation(coord, target_coord) if self.rope else {}
         for block in self.decoder_blocks:
-            x = block(x)
+            x = block(x, **rotation)
         return self.decoder_head(self.decoder_norm(x[:, -m:]))
 
     def forward(self, images: Tensor, mask: Tensor, num_visible: int, num_predict: Optional[int] = None,
@@ -174,7 +194,7 @@ class ViTMAE3D(nn.Module):
         vis_mask, target_mask = torch.split(mask_patches, [num_visible, num_predict], dim=1)
         vis_coord, target_coord = torch.split(coord, [num_visible, num_predict], dim=1)
         embeds = self.forward_encoder(vis_patches, vis_coord)
-        pred = self.forward_decoder(embeds, target_coord)
+        pred = self.forward_decoder(embeds, target_coord, coord=vis_coord)
         loss = F.mse_loss(pred, target_patches, reduction="none")
         loss = (target_mask * loss).sum() / target_mask.sum()
         if not with_state:
@@ -227,10 +247,15 @@ class ViTMAE3D(nn.Module):
             new_seq[dest] = seq_id
             new_seq[cls_rows] = torch.arange(n, device=tokens.device).repeat_interleave(r)
             seq_id = new_seq
+            if self.rope:
+                moved = coord.new_zeros(t + r * n, coord.shape[1])  # class tokens stand at the origin
+                moved[dest] = coord
+                coord = moved
             cu_seqlens = (cu_seqlens.to(torch.int64) + r * torch.arange(n + 1, device=tokens.device)).to(torch.int32)
             max_seqlen = max_seqlen + r
+        rotation = {"coord": coord} if self.rope else {}
         for block in self.blocks:
-            x = block(x, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, seq_id=seq_id)
+            x = block(x, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, seq_id=seq_id, **rotation)
         return self.norm(x), cu_seqlens, max_seqlen, seq_id, is_cls
 
     def forward_packed(self, images: Tensor, mask: Tensor, counts: Tensor, max_visible: int,
@@ -272,8 +297,9 @@ class ViTMAE3D(nn.Module):
         mask_tokens = self.decoder_pos_embed(self.mask_token.expand(n, seq_length, -1), seq_coord)
         mask_tokens = torch.cat([mask_tokens.new_zeros(n, r, mask_tokens.shape[2]), mask_tokens], dim=1)
         y = torch.where(from_enc[:, :, None], dense_enc.to(mask_tokens.dtype), mask_tokens)
+        rotation = self._rotation(seq_coord)  # (row R + j holds patch j of the order, visible or masked)
         for block in self.decoder_blocks:
-            y = block(y)
+            y = block(y, **rotation)
         pred = self.decoder_head(self.decoder_norm(y[:, r:]))            # [N, seq_length, P]
 
         target = patches[bid, order].flatten(0, 1)
@@ -349,6 +375,8 @@ class ViTMAE3D(nn.Module):
         heads = None
         for blk in self.blocks:
             if not (_plain(blk, Block) and _plain(blk.attn, Attention) and _plain(blk.mlp, Mlp)):
+                return None
+            if blk.attn.q_norm is not None:
                 return None
             n1, attn, n2, mlp, act = blk.norm1, blk.attn, blk.norm2, blk.mlp, blk.mlp.act
             linears = (attn.q, attn.k, attn.v, attn.proj, mlp.fc1, mlp.fc2)

@@ -6,17 +6,22 @@
 (``src/nanobrain/modules.py:21-65``). It adds a packed path: given ``[T, dim]`` tokens of several
 sequences and their ``cu_seqlens`` it views the Linear outputs as ``[T, H, 64]`` -- already the
 varlen layout, no copy -- and calls the varlen operator.
+
+What the reference's blocks do not have is off by default: norms of queries and keys and their rotation by the
+tokens' grid coordinates (``Attention(qk_norm=True, rope_grid=...)``), and a gated MLP (:class:`GatedMlp`,
+``Block(mlp="swiglu")``).
 """
 
 from __future__ import annotations
 
 from functools import partial
-from typing import Callable, Optional, Tuple
+from typing import Callable, Optional, Sequence, Tuple
 
 import torch
 import torch.nn as nn
 from torch import Tensor
 
+from .block_ops import gated_mlp, qk_norm_rope
 from .ops import sdpa, sdpa_varlen
 
 # The reference's norm layer: LayerNorm with timm's eps (``src/nanobrain/modules.py:88-89``).
@@ -52,8 +57,27 @@ class DropPath(nn.Module):
         return x * mask
 
 
+def axial_frequencies(grid: Sequence[int], head_dim: int = 64) -> Tensor:
+    """Frequencies ``[len(grid), head_dim // 2]`` that rotate a head's pairs by a token's grid coordinates: the
+    pairs are dealt out to the axes in equal runs, and an axis of ``n`` places has a geometric series of frequencies
+    from 1 down to about ``1 / n``, so that the slowest pairs turn by about one radian over the grid. For
+    :func:`nanobrain_b200.qk_norm_rope`."""
+    pairs = head_dim // 2
+    axes = len(grid)
+    per = -(-pairs // axes)
+    pair = torch.arange(pairs)
+    extent = torch.tensor([float(n) for n in grid], dtype=torch.float64)
+    freqs = torch.zeros(axes, pairs, dtype=torch.float64)
+    freqs[pair // per, pair] = extent[pair // per] ** (-(pair % per).to(torch.float64) / per)
+    return freqs.to(torch.float32)
+
+
 class Attention(nn.Module):
-    """Multi-head bidirectional attention; drop-in for ``nanobrain.modules.Attention``."""
+    """Multi-head bidirectional attention; drop-in for ``nanobrain.modules.Attention``.
+
+    ``qk_norm`` adds an RMS norm of every head's queries and keys (weights ``q_norm``, ``k_norm``), ``rope_grid``
+    the rotation by token coordinates on a grid of that size (``coord`` of :meth:`forward`); both are one pass in front
+    of the attention operator."""
 
     def __init__(
         self,
@@ -63,8 +87,12 @@ class Attention(nn.Module):
         proj_bias: bool = False,
         context_dim: Optional[int] = None,
         causal: bool = False,
+        qk_norm: bool = False,
+        rope_grid: Optional[Sequence[int]] = None,
     ) -> None:
         super().__init__()
+        if rope_grid is not None and not qk_norm:
+            raise ValueError("rope_grid needs qk_norm: norms and rotation are one operator")
         if causal:
             raise ValueError("the B200 attention operator is bidirectional only (the reference never sets causal)")
         if dim % num_heads != 0 or dim // num_heads != 64:
@@ -77,9 +105,22 @@ class Attention(nn.Module):
         self.k = nn.Linear(kv_in, dim, bias=qkv_bias)
         self.v = nn.Linear(kv_in, dim, bias=qkv_bias)
         self.proj = nn.Linear(dim, dim, bias=proj_bias)
+        self.q_norm = nn.Parameter(torch.ones(self.head_dim)) if qk_norm else None
+        self.k_norm = nn.Parameter(torch.ones(self.head_dim)) if qk_norm else None
+        self.register_buffer("rope_freqs", None if rope_grid is None else axial_frequencies(rope_grid), persistent=False)
 
     def extra_repr(self) -> str:
         return f"num_heads={self.num_heads}, causal={self.causal}"
+
+    def _norm_rope(self, q: Tensor, k: Tensor, coord: Optional[Tensor], context_coord: Optional[Tensor]) -> Tuple[Tensor, Tensor]:
+        if self.q_norm is None:
+            return q, k
+        if self.rope_freqs is None:
+            coord = context_coord = None
+        elif coord is None:
+            raise ValueError("coord is required: this attention rotates queries and keys by their tokens' coordinates")
+        return qk_norm_rope(q, k, self.q_norm, self.k_norm, positions=coord, freqs=self.rope_freqs,
+                            k_positions=context_coord)
 
     def forward(
         self,
@@ -89,8 +130,14 @@ class Attention(nn.Module):
         max_seqlen: Optional[int] = None,
         cu_seqlens_k: Optional[Tensor] = None,
         max_seqlen_k: Optional[int] = None,
+        coord: Optional[Tensor] = None,
+        context_coord: Optional[Tensor] = None,
     ) -> Tensor:
+        """``coord``: the tokens' grid coordinates, ``[B, N, axes]`` or packed ``[T, axes]``, where the module rotates;
+        ``context_coord``: those of ``context``."""
         src = x if context is None else context
+        if context is not None and context_coord is None and self.rope_freqs is not None:
+            raise ValueError("context_coord is required with context: its tokens have coordinates of their own")
         heads, hd = self.num_heads, self.head_dim
         if cu_seqlens is None:
             # Dense: x [B, N, dim]; views of the Linear outputs, logical [B, H, N, 64].
@@ -99,6 +146,7 @@ class Attention(nn.Module):
             q = self.q(x).view(bsz, n, heads, hd).transpose(1, 2)
             k = self.k(src).view(bsz, m, heads, hd).transpose(1, 2)
             v = self.v(src).view(bsz, m, heads, hd).transpose(1, 2)
+            q, k = self._norm_rope(q, k, coord, context_coord)
             y = sdpa(q, k, v, is_causal=False)
             y = y.transpose(1, 2).reshape(bsz, n, dim)
         else:
@@ -111,6 +159,7 @@ class Attention(nn.Module):
             q = self.q(x).view(t, heads, hd)
             k = self.k(src).view(src.shape[0], heads, hd)
             v = self.v(src).view(src.shape[0], heads, hd)
+            q, k = self._norm_rope(q, k, coord, context_coord)
             y = sdpa_varlen(q, k, v, cu_seqlens, cu_k, max_seqlen, max_k).reshape(t, dim)
         return self.proj(y)
 
@@ -129,23 +178,63 @@ class Mlp(nn.Module):
         return self.fc2(self.act(self.fc1(x)))
 
 
+class GatedMlp(nn.Module):
+    """Token-wise gated MLP: ``fc2(act(fc_gate(x)) * fc_up(x))`` in two kernels (:func:`nanobrain_b200.gated_mlp`), in the
+    place of :class:`Mlp`. Its hidden width is two thirds of the MLP's, up to a multiple of 8, so that it has as many
+    parameters. ``checkpoint`` says in how many bits the activations are kept for the backward. Under autocast the
+    parameters are cast as those of ``nn.Linear`` are; the three Linears hold them and are not called."""
+
+    def __init__(self, dim: int, mlp_ratio: float = 4, bias: bool = False, activation: str = "silu",
+                 checkpoint: str = "16bit") -> None:
+        super().__init__()
+        hidden = -(-int(dim * mlp_ratio * 2 / 3) // 8) * 8
+        self.activation = activation
+        self.checkpoint = checkpoint
+        self.fc_gate = nn.Linear(dim, hidden, bias=bias)
+        self.fc_up = nn.Linear(dim, hidden, bias=bias)
+        self.fc2 = nn.Linear(hidden, dim, bias=bias)
+
+    def extra_repr(self) -> str:
+        return f"activation={self.activation}, checkpoint={self.checkpoint}"
+
+    def forward(self, x: Tensor) -> Tensor:
+        layers = (self.fc_gate, self.fc_up, self.fc2)
+        args = [x] + [m.weight for m in layers] + [m.bias for m in layers]
+        if torch.is_autocast_enabled("cuda"):
+            dtype = torch.get_autocast_dtype("cuda")
+            args = [t if t is None else t.to(dtype) for t in args]
+        return gated_mlp(*args, activation=self.activation, checkpoint=self.checkpoint)
+
+
+def _make_mlp(kind: str, dim: int, mlp_ratio: float, bias: bool, checkpoint: str) -> nn.Module:
+    if kind == "gelu":
+        return Mlp(dim, mlp_ratio=mlp_ratio, bias=bias)
+    if kind in ("swiglu", "geglu"):
+        return GatedMlp(dim, mlp_ratio=mlp_ratio, bias=bias, activation="silu" if kind == "swiglu" else "gelu",
+                        checkpoint=checkpoint)
+    raise ValueError(f"mlp must be 'gelu', 'swiglu' or 'geglu', got {kind!r}")
+
+
 class Block(nn.Module):
     """Pre-norm residual block, drop-in for ``nanobrain.modules.Block``
     (``src/nanobrain/modules.py:92-131``): same constructor arguments -- the reference builds its
     encoder with ``Block(..., drop_path=dpr[ii])`` at ``src/nanobrain/model.py:68-75`` -- and the
     same parameter names. ``cu_seqlens`` / ``max_seqlen`` are passed through to the attention, so
     one block serves dense ``[B, N, dim]`` and packed ``[T, dim]`` tokens (LayerNorm and the MLP
-    are token-wise); with stochastic depth on packed tokens also pass ``seq_id``."""
+    are token-wise); with stochastic depth on packed tokens also pass ``seq_id``. ``qk_norm``, ``rope_grid`` (with
+    ``coord`` in the call), ``mlp`` and ``mlp_checkpoint`` choose what the reference does not have."""
 
     def __init__(self, dim: int, num_heads: int, qkv_bias: bool = False, proj_bias: bool = False,
                  context_dim: Optional[int] = None, mlp_ratio: float = 4, drop_path: float = 0.0,
-                 norm_layer: Callable[[int], nn.Module] = LayerNorm) -> None:
+                 norm_layer: Callable[[int], nn.Module] = LayerNorm, qk_norm: bool = False,
+                 rope_grid: Optional[Sequence[int]] = None, mlp: str = "gelu", mlp_checkpoint: str = "16bit") -> None:
         super().__init__()
         self.norm1 = norm_layer(dim)
-        self.attn = Attention(dim, num_heads, qkv_bias=qkv_bias, proj_bias=proj_bias, context_dim=context_dim)
+        self.attn = Attention(dim, num_heads, qkv_bias=qkv_bias, proj_bias=proj_bias, context_dim=context_dim,
+                              qk_norm=qk_norm, rope_grid=rope_grid)
         self.drop_path1 = DropPath(drop_path) if drop_path > 0 else nn.Identity()
         self.norm2 = norm_layer(dim)
-        self.mlp = Mlp(dim, mlp_ratio=mlp_ratio, bias=proj_bias)
+        self.mlp = _make_mlp(mlp, dim, mlp_ratio, proj_bias, mlp_checkpoint)
         self.drop_path2 = DropPath(drop_path) if drop_path > 0 else nn.Identity()
 
     def _drop(self, layer: nn.Module, y: Tensor, seq_id: Optional[Tensor], num_seqs: Optional[int]) -> Tensor:
@@ -154,9 +243,11 @@ class Block(nn.Module):
         return layer(y)
 
     def forward(self, x: Tensor, context: Optional[Tensor] = None, cu_seqlens: Optional[Tensor] = None,
-                max_seqlen: Optional[int] = None, seq_id: Optional[Tensor] = None) -> Tensor:
+                max_seqlen: Optional[int] = None, seq_id: Optional[Tensor] = None, coord: Optional[Tensor] = None,
+                context_coord: Optional[Tensor] = None) -> Tensor:
         num_seqs = None if cu_seqlens is None else cu_seqlens.numel() - 1
-        y = self.attn(self.norm1(x), context=context, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen)
+        rotation = {} if coord is None else {"coord": coord, "context_coord": context_coord}
+        y = self.attn(self.norm1(x), context=context, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, **rotation)
         x = x + self._drop(self.drop_path1, y, seq_id, num_seqs)
         return x + self._drop(self.drop_path2, self.mlp(self.norm2(x)), seq_id, num_seqs)
 
