@@ -284,28 +284,27 @@ size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Teams of one or two CTAs, and the columns of their tiles, by the clocks that a team's share of the tiles takes. A 64-deep
 // step's MMAs take two clocks a column; its operands cross the port of a CTA's shared memory (128 bytes a clock) twice.
-// A tile also costs its epilogue's start and end, of which the last one of a team is not hidden.
+// A tile's epilogue takes `epilogue` clocks a column and runs under the next tile's products; the last one does not.
 struct Tiling {
   int ctas, cols, row_tiles, col_tiles;
   double clocks;
 };
+constexpr double kPlainClocks = 8, kGateClocks = 26, kDactClocks = 30;  // per column and CTA
 double step_clocks(const Tiling& t) { return std::max(2.0 * t.cols, 256.0 + 2.0 * t.cols / t.ctas); }
-Tiling tiling(int64_t m, int n, int steps, int sms, int ctas, int cols) {
+Tiling tiling(int64_t m, int n, int steps, int sms, int ctas, int cols, double epilogue) {
   Tiling t{ctas, cols, div_up(m, int64_t(ctas) * kGemmRows), div_up(n, cols), 0.0};
   const int64_t tiles = int64_t(t.row_tiles) * t.col_tiles, teams = sms / ctas;
-  t.clocks = double((tiles + teams - 1) / teams) * (steps * step_clocks(t) + 400.0) + 2.0 * cols + 1000.0 * ctas;
+  t.clocks = double((tiles + teams - 1) / teams) * (std::max(steps * step_clocks(t), epilogue * cols) + 400.0) + epilogue * cols +
+             1000.0 * ctas;
   return t;
 }
-// Widths are multiples of 64 per CTA, and of `unit`.
-Tiling best_tiling(int64_t m, int n, int steps, int sms, int unit) {
-  Tiling best = tiling(m, n, steps, sms, 2, kGemmMaxCols);
-  for (int ctas = 2; ctas >= 1; --ctas) {
-    const int by = std::max(unit, 64 * ctas);
-    for (int cols = kGemmMaxCols; cols >= by; cols -= by) {
-      const Tiling t = tiling(m, n, steps, sms, ctas, cols);
+Tiling best_tiling(int64_t m, int n, int steps, int sms, double epilogue) {
+  Tiling best = tiling(m, n, steps, sms, 2, kGemmMaxCols, epilogue);
+  for (int ctas = 2; ctas >= 1; --ctas)
+    for (int cols = kGemmMaxCols; cols >= 64; cols -= 64) {
+      const Tiling t = tiling(m, n, steps, sms, ctas, cols, epilogue);
       if (t.clocks < 0.98 * best.clocks) best = t;
     }
-  }
   return best;
 }
 
@@ -405,10 +404,10 @@ struct BwdPlan {
 // The products behind da and db by teams of `ctas`; parts[] receives the bytes that are needed there.
 BwdPlan plan_products(BwdPlan p, const nb_gated_mlp_bwd_args& a, int sms, int ctas) {
   const nb_gated_mlp_shape& s = a.shape;
-  const int dx_steps = 2 * div_up(s.hidden, kGemmDepth), dw_steps = div_up(s.tokens, kGemmDepth), unit = 64 * ctas;
+  const int dx_steps = 2 * div_up(s.hidden, kGemmDepth), dw_steps = div_up(s.tokens, kGemmDepth);
   const bool wanted[3] = {a.d_w_gate.ptr != nullptr, a.d_w_up.ptr != nullptr, a.d_w_down.ptr != nullptr};
-  const auto width = [unit](int n) { return std::min(kGemmMaxCols, div_up(div_up(n, div_up(n, kGemmMaxCols)), unit) * unit); };
-  p.dx = tiling(s.tokens, s.dim, dx_steps, sms, ctas, width(s.dim));
+  const auto width = [](int n) { return div_up(div_up(n, div_up(n, kGemmMaxCols)), 64) * 64; };
+  p.dx = tiling(s.tokens, s.dim, dx_steps, sms, ctas, width(s.dim), kPlainClocks);
   double total = 0.0, longest = 0.0;
   if (a.dx.ptr != nullptr) {
     longest = step_clocks(p.dx) * dx_steps;
@@ -416,7 +415,7 @@ BwdPlan plan_products(BwdPlan p, const nb_gated_mlp_bwd_args& a, int sms, int ct
   }
   for (int i = 0; i < 3; ++i) {
     const int m = i < 2 ? s.hidden : s.dim, n = i < 2 ? s.dim : s.hidden;
-    p.dw[i] = tiling(m, n, dw_steps, sms, ctas, width(n));
+    p.dw[i] = tiling(m, n, dw_steps, sms, ctas, width(n), kPlainClocks);
     if (wanted[i]) total += step_clocks(p.dw[i]) * p.dw[i].row_tiles * p.dw[i].col_tiles * dw_steps;
   }
   // A weight gradient's unit runs over all tokens. Where that is more than a team's even share of the launch's work, it is
@@ -426,7 +425,8 @@ BwdPlan plan_products(BwdPlan p, const nb_gated_mlp_bwd_args& a, int sms, int ct
     const double steps = share / step_clocks(p.dw[i]);
     int splits = 1;
     if (dw_steps > 0.8 * steps) splits = std::min(div_up(dw_steps, 8), int(dw_steps / std::max(0.5 * steps, 8.0)) + 1);
-    splits = std::max(1, std::min(splits, 32));
+    // (and a unit stays far below the time after which a wait gives up)
+    splits = std::max({1, std::min(splits, 32), div_up(dw_steps, 1 << 18)});
     p.split_steps[i] = div_up(dw_steps, splits);
     p.splits[i] = div_up(dw_steps, p.split_steps[i]);
     const size_t tiles = size_t(p.dw[i].row_tiles) * ctas * p.dw[i].col_tiles;
@@ -493,8 +493,8 @@ extern "C" int nb_gated_mlp_fwd(const nb_gated_mlp_fwd_args* args, void* stream)
   const int steps = div_up(s.dim, kGemmDepth);
   GemmParams<1> g{};
   GemmProblem& p = g.p[0];
-  // (a tile has as many columns of a as of b, 64 at least)
-  const Tiling tg = best_tiling(s.tokens, 2 * s.hidden, steps, sms, 128);
+  // (a tile has as many columns of a as of b)
+  const Tiling tg = best_tiling(s.tokens, 2 * s.hidden, steps, sms, kGateClocks);
   const int cols = tg.cols;
   set_tiles(&p, s.tokens, s.hidden, tg, steps, steps);
   p.col_tiles = div_up(s.hidden, cols / 2);
@@ -512,7 +512,7 @@ extern "C" int nb_gated_mlp_fwd(const nb_gated_mlp_fwd_args* args, void* stream)
   GemmParams<1> d{};
   GemmProblem& q = d.p[0];
   const int down_steps = div_up(s.hidden, kGemmDepth);
-  const Tiling td = best_tiling(s.tokens, s.dim, down_steps, sms, 64);
+  const Tiling td = best_tiling(s.tokens, s.dim, down_steps, sms, kPlainClocks);
   set_tiles(&q, s.tokens, s.dim, td, down_steps, down_steps);
   NB_TRY(map_k_major(&q.a[0], args->h, s.tokens, s.hidden, kGemmRows));
   NB_TRY(map_k_major(&q.b[0], args->w_down, s.dim, s.hidden, td.cols / td.ctas));
@@ -570,7 +570,7 @@ extern "C" int nb_gated_mlp_bwd(const nb_gated_mlp_bwd_args* args, void* stream)
     GemmParams<1>& g = act;
     GemmProblem& p = g.p[0];
     const int steps = div_up(s.dim, kGemmDepth);
-    act_tiling = best_tiling(s.tokens, s.hidden, steps, sms, 64);
+    act_tiling = best_tiling(s.tokens, s.hidden, steps, sms, kDactClocks);
     set_tiles(&p, s.tokens, s.hidden, act_tiling, steps, steps);
     p.b_mn = 1;
     NB_TRY(map_k_major(&p.a[0], a.dy, s.tokens, s.dim, kGemmRows));

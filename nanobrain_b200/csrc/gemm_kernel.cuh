@@ -379,7 +379,9 @@ __global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas>::kThreads, 1)
         const GemmProblem& p = g.p[u.problem];
         const int cols = p.cols, mine = cols / kCtas;  // columns of the tile, and those that this CTA loads
         const int row0 = (u.row * kCtas + rank) * kGemmRows, col0 = u.col * cols + rank * mine;
-        const uint32_t bytes = kCtas * (kGemmBytesA + uint32_t(mine) * (kGemmDepth * 2));
+        // (B's tile in blocks of 64 columns where its columns run along memory: a pair's 96 take two blocks)
+        const int loaded = p.b_mn ? (mine + 63) / 64 * 64 : mine;
+        const uint32_t bytes = kCtas * (kGemmBytesA + uint32_t(loaded) * (kGemmDepth * 2));
         for (int s = u.begin; s < u.end; ++s) {
           mbar_wait(empty + 8 * stage, phase ^ 1, abort_flag);
           const uint32_t at_a = base + stage * L::kStageBytes, at_b = at_a + kGemmBytesA;
@@ -403,7 +405,7 @@ __global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas>::kThreads, 1)
               load(at_b + half * 128, &p.b[1], bar, k, u.col * half);
             }
           } else if (p.b_mn) {
-            for (int b = 0; b < mine / 64; ++b) load(at_b + b * 8192, &p.b[second], bar, col0 + b * 64, k);
+            for (int b = 0; b < loaded / 64; ++b) load(at_b + b * 8192, &p.b[second], bar, col0 + b * 64, k);
           } else {
             load(at_b, &p.b[second], bar, k, col0);
           }

@@ -9,6 +9,7 @@
 #include <torch/library.h>
 
 #include <array>
+#include <cmath>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -120,6 +121,7 @@ QkCall make_call(const Tensor& q, const Tensor& k, const MaybeTensor& q_weight, 
   c.args.interleaved = interleaved;
   c.args.eps = float(eps);
   c.args.position_type = -1;
+  QK_REQUIRE(eps >= 0.0 && std::isfinite(eps), "eps must be finite and not negative, got ", eps);
   QK_REQUIRE(has(positions) == has(freqs), "positions and freqs come together");
   QK_REQUIRE(!has(k_positions) || has(positions), "k_positions need positions");
   if (has(freqs)) {
@@ -293,8 +295,8 @@ Three mlp_fwd_cuda(const Tensor& x_, const Tensor& w_gate_, const Tensor& w_up_,
   a.shape = {tokens, int32_t(dim), int32_t(hidden), int32_t(activation), int32_t(checkpoint)};
   Tensor y = new_tensor(x_.sizes(), at::kBFloat16, x), h = new_tensor({tokens, padded(hidden)}, at::kBFloat16, x);
   Tensor codes = new_tensor({int64_t(nb_gated_mlp_checkpoint_bytes(&a.shape))}, at::kByte, x);
-  const auto result = [&]() -> Three {  // in 8 bits the backward makes h again
-    return {y, checkpoint == NB_CHECKPOINT_8BIT ? new_tensor({0}, at::kBFloat16, x) : h.narrow(1, 0, hidden), codes};
+  const auto result = [&]() -> Three {  // the backward wants h from 16 bits; in 8 bits it makes h again
+    return {y, checkpoint == NB_CHECKPOINT_16BIT ? h.narrow(1, 0, hidden) : new_tensor({0}, at::kBFloat16, x), codes};
   };
   if (tokens == 0) return result();
   a.x = matrix(x), a.w_gate = matrix(w_gate), a.w_up = matrix(w_up), a.w_down = matrix(w_down);
