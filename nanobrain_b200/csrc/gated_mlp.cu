@@ -386,9 +386,20 @@ int launch_act(const GemmParams<1>& g, const nb_gated_mlp_shape& s, int ctas, in
                                      : launch_bits<kKind, kActGelu>(g, s.checkpoint, ctas, sms, stream);
 }
 
+// The kernels divide unit numbers (below 2^31) by the column tiles: with 2^(k-1) < d <= 2^k, ceil(2^(31+k) / d) is below 2^32
+// and its product's excess, below u / 2^31, does not reach the next whole number.
+void set_col_tiles(GemmProblem* p, int col_tiles) {
+  int k = 0;
+  while ((int64_t(1) << k) < col_tiles) ++k;
+  p->col_tiles = col_tiles;
+  p->by_shift = uint32_t(31 + k);
+  p->by_col_tiles = uint32_t(((uint64_t(1) << (31 + k)) + col_tiles - 1) / col_tiles);
+}
+
 void set_tiles(GemmProblem* p, int64_t rows, int n, const Tiling& t, int steps0, int steps) {
   p->m = int(rows), p->n = n;
-  p->row_tiles = t.row_tiles, p->col_tiles = t.col_tiles, p->cols = t.cols;
+  p->row_tiles = t.row_tiles, p->cols = t.cols;
+  set_col_tiles(p, t.col_tiles);
   p->steps0 = steps0, p->steps = steps;
   p->splits = 1, p->split_steps = steps;
 }
@@ -497,7 +508,7 @@ extern "C" int nb_gated_mlp_fwd(const nb_gated_mlp_fwd_args* args, void* stream)
   const Tiling tg = best_tiling(s.tokens, 2 * s.hidden, steps, sms, kGateClocks);
   const int cols = tg.cols;
   set_tiles(&p, s.tokens, s.hidden, tg, steps, steps);
-  p.col_tiles = div_up(s.hidden, cols / 2);
+  set_col_tiles(&p, div_up(s.hidden, cols / 2));
   NB_TRY(map_k_major(&p.a[0], args->x, s.tokens, s.dim, kGemmRows));
   NB_TRY(map_k_major(&p.b[0], args->w_gate, s.hidden, s.dim, cols / 2));
   NB_TRY(map_k_major(&p.b[1], args->w_up, s.hidden, s.dim, cols / 2));

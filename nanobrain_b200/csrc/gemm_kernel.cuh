@@ -59,6 +59,7 @@ struct GemmProblem {
   float* partial;             // [split][row tile][column tile][columns / 4][128 rows][4], where splits > 1
   int32_t m, n;               // rows and columns of the output
   int32_t row_tiles, col_tiles, cols;  // tiles of 128 rows per CTA of the team; cols: of a tile
+  uint32_t by_col_tiles, by_shift;     // u / col_tiles = u * by_col_tiles >> by_shift for u < 2^31
   int32_t steps0, steps;      // 64-deep steps of the first range, of both
   int32_t splits, split_steps;
   int32_t a_mn, b_mn;         // the operand's inner index does not run along memory
@@ -69,20 +70,30 @@ struct GemmProblem {
 // the rest of the short units goes round again.
 struct GemmDeal {
   int32_t n_long, n_short, extra;
-  template <int kCtas>
-  __device__ __forceinline__ int unit(int i) const {  // -1: no more
-    const int g = int(gridDim.x) / kCtas, me = int(blockIdx.x) / kCtas;
-    const int mine = me < n_long ? (n_long - me + g - 1) / g : 0;
-    if (i < mine) return me + i * g;
-    int j = i - mine;
-    const int rem = n_long % g;
-    if (me >= rem) {
-      if (j < extra) return n_long + (me - rem) * extra + j;
-      j -= extra;
+};
+template <int kCtas>
+struct GemmTurns {
+  int team, teams, n_long, n_short, mine, extra, rest;  // long units of this team; where its other short units begin
+  __device__ __forceinline__ explicit GemmTurns(const GemmDeal& d) {
+    teams = int(gridDim.x) / kCtas, team = int(blockIdx.x) / kCtas;
+    n_long = d.n_long, n_short = d.n_short;
+    mine = extra = 0, rest = team;
+    if (n_long > 0) {
+      const int rem = n_long % teams;
+      mine = n_long / teams + (team < rem);
+      if (team >= rem) extra = d.extra;
+      rest = (teams - rem) * d.extra + team;
+      first_extra = n_long + (team - rem) * d.extra;
     }
-    const int at = (g - rem) * extra + me + j * g;
+  }
+  __device__ __forceinline__ int unit(int i) const {  // the i-th of this team; -1: no more
+    if (i < mine) return team + i * teams;
+    i -= mine;
+    if (i < extra) return first_extra + i;
+    const int at = rest + (i - extra) * teams;
     return at < n_short ? n_long + at : -1;
   }
+  int first_extra = 0;
 };
 
 template <int kProblems>
@@ -122,7 +133,7 @@ __device__ __forceinline__ GemmUnit gemm_unit(const GemmParams<kProblems>& g, in
     r.split = u / tiles;
     u -= r.split * tiles;
   }
-  r.row = u / p.col_tiles;
+  r.row = int(uint64_t(uint32_t(u)) * p.by_col_tiles >> p.by_shift);
   r.col = u - r.row * p.col_tiles;
   r.begin = r.split * p.split_steps;
   r.end = min(r.begin + p.split_steps, p.steps);
@@ -143,58 +154,59 @@ __device__ __forceinline__ float fast_rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ uint64_t both(float v) { return pack_f32x2(v, v); }
-__device__ __forceinline__ uint64_t exp2_of(uint64_t v) {
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ void split(float2 v, float& x, float& y) { x = v.x, y = v.y; }
+__device__ __forceinline__ float2 exp2_of(float2 v) {
   float x, y;
-  unpack_f32x2(v, x, y);
-  return pack_f32x2(fast_exp2(x), fast_exp2(y));
+  split(v, x, y);
+  return make_float2(fast_exp2(x), fast_exp2(y));
 }
-__device__ __forceinline__ uint64_t rcp_of(uint64_t v) {
+__device__ __forceinline__ float2 rcp_of(float2 v) {
   float x, y;
-  unpack_f32x2(v, x, y);
-  return pack_f32x2(fast_rcp(x), fast_rcp(y));
+  split(v, x, y);
+  return make_float2(fast_rcp(x), fast_rcp(y));
 }
 // 1 / (1 + e^-a), or Phi(a) with e = e^(-a^2 / 2).
-__device__ __forceinline__ uint64_t sigmoid_of(uint64_t a) {
-  return rcp_of(add_f32x2(exp2_of(mul_f32x2(a, both(-1.4426950408889634f))), both(1.f)));
+__device__ __forceinline__ float2 sigmoid_of(float2 a) {
+  return rcp_of(__fadd2_rn(exp2_of(__fmul2_rn(a, both(-1.4426950408889634f))), both(1.f)));
 }
-__device__ __forceinline__ uint64_t phi_of(uint64_t a, uint64_t& e) {
-  const uint64_t mag = a & 0x7FFFFFFF7FFFFFFFull;
-  const uint64_t t = rcp_of(fma_f32x2(mag, both(0.3275911f * 0.70710678118654752f), both(1.f)));
-  e = exp2_of(mul_f32x2(mul_f32x2(a, both(-0.72134752044448170f)), a));
-  uint64_t q = fma_f32x2(t, both(1.061405429f), both(-1.453152027f));
-  q = fma_f32x2(t, q, both(1.421413741f));
-  q = fma_f32x2(t, q, both(-0.284496736f));
-  q = fma_f32x2(t, q, both(0.254829592f));
-  q = mul_f32x2(mul_f32x2(t, both(0.5f)), mul_f32x2(q, e));  // Phi(-|a|)
+__device__ __forceinline__ float2 phi_of(float2 a, float2& e) {
+  const float2 mag = make_float2(fabsf(a.x), fabsf(a.y));
+  const float2 t = rcp_of(__ffma2_rn(mag, both(0.3275911f * 0.70710678118654752f), both(1.f)));
+  e = exp2_of(__fmul2_rn(__fmul2_rn(a, both(-0.72134752044448170f)), a));
+  float2 q = __ffma2_rn(t, both(1.061405429f), both(-1.453152027f));
+  q = __ffma2_rn(t, q, both(1.421413741f));
+  q = __ffma2_rn(t, q, both(-0.284496736f));
+  q = __ffma2_rn(t, q, both(0.254829592f));
+  q = __fmul2_rn(__fmul2_rn(t, both(0.5f)), __fmul2_rn(q, e));  // Phi(-|a|)
   float x, y, qx, qy;
-  unpack_f32x2(a, x, y);
-  unpack_f32x2(q, qx, qy);
-  return pack_f32x2(x < 0.f ? qx : 1.f - qx, y < 0.f ? qy : 1.f - qy);
+  split(a, x, y);
+  split(q, qx, qy);
+  return make_float2(x < 0.f ? qx : 1.f - qx, y < 0.f ? qy : 1.f - qy);
 }
 template <int kAct>
-__device__ __forceinline__ uint64_t gate_of(uint64_t a) {
-  uint64_t e;
-  if constexpr (kAct == kActSilu) return mul_f32x2(a, sigmoid_of(a));
-  else return mul_f32x2(a, phi_of(a, e));
+__device__ __forceinline__ float2 gate_of(float2 a) {
+  float2 e;
+  if constexpr (kAct == kActSilu) return __fmul2_rn(a, sigmoid_of(a));
+  else return __fmul2_rn(a, phi_of(a, e));
 }
 template <int kAct>
-__device__ __forceinline__ void gate_and_slope(uint64_t a, uint64_t& gate, uint64_t& slope) {
+__device__ __forceinline__ void gate_and_slope(float2 a, float2& gate, float2& slope) {
   if constexpr (kAct == kActSilu) {
-    const uint64_t s = sigmoid_of(a);
-    gate = mul_f32x2(a, s);
-    slope = fma_f32x2(gate, fma_f32x2(s, both(-1.f), both(1.f)), s);
+    const float2 s = sigmoid_of(a);
+    gate = __fmul2_rn(a, s);
+    slope = __ffma2_rn(gate, __ffma2_rn(s, both(-1.f), both(1.f)), s);
   } else {
-    uint64_t e;
-    const uint64_t phi = phi_of(a, e);
-    gate = mul_f32x2(a, phi);
-    slope = fma_f32x2(mul_f32x2(a, both(0.39894228040143268f)), e, phi);
+    float2 e;
+    const float2 phi = phi_of(a, e);
+    gate = __fmul2_rn(a, phi);
+    slope = __ffma2_rn(__fmul2_rn(a, both(0.39894228040143268f)), e, phi);
   }
 }
 template <int kAct>
 __device__ __forceinline__ float gate_of(float a) {
   float x, y;
-  unpack_f32x2(gate_of<kAct>(both(a)), x, y);
+  split(gate_of<kAct>(both(a)), x, y);
   return x;
 }
 
@@ -224,11 +236,11 @@ __device__ __forceinline__ uint32_t encode(const float (&v)[32], uint32_t (&w)[C
   if constexpr (kBits == 16) {
     uint32_t e = __float_as_uint(m) >> 23;
     e = e == 255u ? 141u : max(e, 15u);
-    const uint64_t inv = both(__uint_as_float((268u - e) << 23));
+    const float2 inv = both(__uint_as_float((268u - e) << 23));
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float x, y;
-      unpack_f32x2(mul_f32x2(pack_f32x2(v[2 * i], v[2 * i + 1]), inv), x, y);
+      split(__fmul2_rn(make_float2(v[2 * i], v[2 * i + 1]), inv), x, y);
       const __half2 h = __floats2half2_rn(x, y);
       w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
@@ -238,14 +250,14 @@ __device__ __forceinline__ uint32_t encode(const float (&v)[32], uint32_t (&w)[C
     float inv = __fdividef(1.f, __uint_as_float(s << 16));
     if (!(m < __uint_as_float(0x7F800000u))) s = 0x7FC0u, inv = 0.f;   // (also NaN)
     else if (s < 0x0D80u) s = 0u, inv = 0.f;                            // below 2^-100: zeros
-    // Adding 1.5 * 2^23 rounds to a whole number, whose low byte is the code.
+    // Adding 1.5 * 2^23 + 128 rounds to a whole number, whose low byte is kept: the code + 128.
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       uint32_t b[4];
 #pragma unroll
       for (int k = 0; k < 4; k += 2) {
         float x, y;
-        unpack_f32x2(fma_f32x2(pack_f32x2(v[4 * i + k], v[4 * i + k + 1]), both(inv), both(12582912.f)), x, y);
+        split(__ffma2_rn(make_float2(v[4 * i + k], v[4 * i + k + 1]), both(inv), both(12583040.f)), x, y);
         b[k] = __float_as_uint(x), b[k + 1] = __float_as_uint(y);
       }
       w[i] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
@@ -256,16 +268,16 @@ __device__ __forceinline__ uint32_t encode(const float (&v)[32], uint32_t (&w)[C
 
 // Values 2 i and 2 i + 1 of a lane's (i known at compile time).
 template <int kBits, int kWords>
-__device__ __forceinline__ uint64_t decode(const uint32_t (&w)[kWords], int i, uint64_t scale) {
+__device__ __forceinline__ float2 decode(const uint32_t (&w)[kWords], int i, float2 scale) {
   if constexpr (kBits == 16) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    return mul_f32x2(pack_f32x2(f.x, f.y), scale);
+    return __fmul2_rn(make_float2(f.x, f.y), scale);
   } else {
-    // The codes with their sign bits turned, in the low byte of 2^23: 2^23 + code + 128.
-    const uint32_t u = w[i >> 1] ^ 0x80808080u;
+    // Put into the low byte of 2^23: 2^23 + 128 + code.
+    const uint32_t u = w[i >> 1];
     const float x = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 | (2 * (i & 1)))),
                 y = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 | (2 * (i & 1) + 1)));
-    return mul_f32x2(add_f32x2(pack_f32x2(x, y), both(-8388736.f)), scale);
+    return __fmul2_rn(__fadd2_rn(make_float2(x, y), both(-8388736.f)), scale);
   }
 }
 
@@ -364,6 +376,7 @@ __global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas>::kThreads, 1)
   uint32_t tmem;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
 
+  const GemmTurns<kCtas> turns(g.deal);
   if (warp == 0) {
     if (lane == 0) {
       const auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
@@ -373,7 +386,7 @@ __global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas>::kThreads, 1)
       int stage = 0;
       uint32_t phase = 0;
       for (int i = 0;; ++i) {
-        const int id = g.deal.template unit<kCtas>(i);
+        const int id = turns.unit(i);
         if (id < 0) break;
         const GemmUnit u = gemm_unit(g, id);
         const GemmProblem& p = g.p[u.problem];
@@ -424,7 +437,7 @@ __global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas>::kThreads, 1)
       int stage = 0;
       uint32_t phase = 0;
       for (int i = 0;; ++i) {
-        const int id = g.deal.template unit<kCtas>(i);
+        const int id = turns.unit(i);
         if (id < 0) break;
         const GemmUnit u = gemm_unit(g, id);
         const GemmProblem& p = g.p[u.problem];
@@ -483,7 +496,7 @@ __global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas>::kThreads, 1)
         ahead.blk += 32 * L::kTeams;
         while (ahead.live && (ahead.i < 0 || ahead.blk >= cols || ahead.u.col * cols + ahead.blk >= g.hidden ||
                               (kPair && rows_of(ahead.u) >= g.p[0].m))) {
-          const int id = g.deal.template unit<kCtas>(++ahead.i);
+          const int id = turns.unit(++ahead.i);
           ahead.live = id >= 0;
           if (ahead.live) ahead.u = gemm_unit(g, id);
           ahead.blk = first_piece(ahead.i, cols / 32);
@@ -498,7 +511,7 @@ __global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas>::kThreads, 1)
     for (int i = 0; i < L::kSlots; ++i) request(i);
 
     for (int i = 0;; ++i) {
-      const int id = g.deal.template unit<kCtas>(i);
+      const int id = turns.unit(i);
       if (id < 0) break;
       const GemmUnit u = gemm_unit(g, id);
       const GemmProblem& p = g.p[u.problem];
@@ -527,7 +540,7 @@ __global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas>::kThreads, 1)
               *reinterpret_cast<uint4*>(block + c * 512 + lane * 16) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
           }
 #pragma unroll
-          for (int k = 0; k < 32; k += 2) unpack_f32x2(gate_of<kAct>(pack_f32x2(a[k], a[k + 1])), a[k], a[k + 1]);
+          for (int k = 0; k < 32; k += 2) split(gate_of<kAct>(make_float2(a[k], a[k + 1])), a[k], a[k + 1]);
           tmem_ld32f(acc + half + blk, b);
           add_bias32(b, g.bias_up, f, g.hidden);
           if constexpr (kBits > 0) {
@@ -556,7 +569,7 @@ __global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas>::kThreads, 1)
           mbar_wait(my_codes + 8 * slot, (piece / L::kSlots) & 1, abort_flag);
           uint32_t scales;
           asm volatile("ld.shared.b32 %0, [%1];" : "=r"(scales) : "r"(codes + Block::kScales + lane * 4) : "memory");
-          const uint64_t sa = both(__uint_as_float(scales << 16)), sb = both(__uint_as_float(scales & 0xFFFF0000u));
+          const float2 sa = both(__uint_as_float(scales << 16)), sb = both(__uint_as_float(scales & 0xFFFF0000u));
           constexpr int kHalf = Block::kChunks / 2;  // chunks of 16 values
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
@@ -578,17 +591,17 @@ __global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas>::kThreads, 1)
             uint32_t vd[8], ve[8], vh[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              const uint64_t a = decode<kB>(wa, k, sa), b = decode<kB>(wb, k, sb),
-                             dh = pack_f32x2(__uint_as_float(r[2 * k]), __uint_as_float(r[2 * k + 1]));
-              uint64_t gate, slope;
+              const float2 a = decode<kB>(wa, k, sa), b = decode<kB>(wb, k, sb),
+                             dh = make_float2(__uint_as_float(r[2 * k]), __uint_as_float(r[2 * k + 1]));
+              float2 gate, slope;
               gate_and_slope<kAct>(a, gate, slope);
-              unpack_f32x2(mul_f32x2(dh, gate), e[2 * k], e[2 * k + 1]);
-              unpack_f32x2(mul_f32x2(mul_f32x2(dh, b), slope), d[2 * k], d[2 * k + 1]);
+              split(__fmul2_rn(dh, gate), e[2 * k], e[2 * k + 1]);
+              split(__fmul2_rn(__fmul2_rn(dh, b), slope), d[2 * k], d[2 * k + 1]);
               vd[k] = pack_bf16(d[2 * k], d[2 * k + 1]);
               ve[k] = pack_bf16(e[2 * k], e[2 * k + 1]);
               if constexpr (kBits == 8) {
                 float x, y;
-                unpack_f32x2(mul_f32x2(gate, b), x, y);
+                split(__fmul2_rn(gate, b), x, y);
                 vh[k] = pack_bf16(x, y);
               }
             }
