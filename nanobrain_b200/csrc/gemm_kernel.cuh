@@ -37,15 +37,16 @@ struct CodeBlock {
   static constexpr int kBytes = kBits ? kScales + 128 : 0;
 };
 
-// Shared memory: stages, then a part for every epilogue warp (a box for TMA's store, or code blocks), then barriers.
-template <int kKind, int kBits, int kCtas>
+// Shared memory: stages, then a part for every epilogue warp (boxes for TMA's stores, code blocks), then barriers.
+template <int kKind, int kBits, int kCtas, bool kSums>
 struct GemmLayout {
   static constexpr int kTeams = kKind == kGemmPlain ? 2 : 3;  // of four warps, for the 128 rows of a tile
   static constexpr int kEpilogueWarps = 4 * kTeams;
   static constexpr int kThreads = 128 + 32 * kEpilogueWarps;
   static constexpr int kStageBytes = kGemmBytesA + kGemmBytesB / kCtas;
-  static constexpr int kSlots = kKind != kGemmDact ? 0 : kBits == 8 ? 2 : 1;  // code blocks under way
-  static constexpr int kWarpBytes = kKind == kGemmPlain ? 4096 : kSlots * CodeBlock<kBits>::kBytes;
+  static constexpr int kSlots = kKind != kGemmDact ? 0 : kBits == 8 && !kSums ? 2 : 1;  // code blocks under way
+  static constexpr int kBoxes = kKind == kGemmPlain ? 4096 : kKind == kGemmDact && kSums ? (kBits == 8 ? 3 : 2) * 2048 : 0;
+  static constexpr int kWarpBytes = (kBoxes + kSlots * CodeBlock<kBits>::kBytes + 511) / 512 * 512;
   static constexpr int kMost = 232448 - 1024 - 512 - kEpilogueWarps * kWarpBytes;
   static constexpr int kStages = kMost / kStageBytes < 6 ? kMost / kStageBytes : 6;
   static constexpr int kWarps = kStages * kStageBytes;
@@ -102,11 +103,12 @@ struct GemmParams {
   GemmDeal deal;
   int32_t* status;
   // the gate's and its backward's
+  CUtensorMap map_db, map_h;   // backward with kSums: and p[0].c of da
   __nv_bfloat16 *da, *db, *h;  // rows of `stride` values, at 32 bytes
   int64_t stride;
   const __nv_bfloat16* bias_up;
   uint8_t* codes;     // checkpoint: [row tile][group][warp] code blocks
-  float* col_sums;    // backward: [row tile][warp][2 x hidden] sums of da and db over 32 rows, or NULL
+  float* col_sums;    // backward with kSums: [row tile][warp][2 x hidden] sums of da and db over 32 rows
   int32_t groups, hidden;
 };
 
@@ -326,6 +328,12 @@ __device__ __forceinline__ void stage_half_row(uint32_t box, int row, int half, 
     st_shared_v4(box + swz128(row, half * 4 + i), pack_bf16(v[8 * i], v[8 * i + 1]), pack_bf16(v[8 * i + 2], v[8 * i + 3]),
                  pack_bf16(v[8 * i + 4], v[8 * i + 5]), pack_bf16(v[8 * i + 6], v[8 * i + 7]));
 }
+// 16 values (`half` of 32) of a row of a box that TMA stores, 32 columns wide, where its swizzle expects them.
+__device__ __forceinline__ void stage_half16(uint32_t box, int row, int half, const uint32_t (&w)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    st_shared_v4(box + row * 64 + (((2 * half + i) ^ ((row >> 1) & 3)) << 4), w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+}
 // 16 values to 32 bytes (a whole sector) of a row.
 __device__ __forceinline__ void store_sector(__nv_bfloat16* p, const uint32_t (&w)[8]) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
@@ -339,10 +347,10 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
 }
 
 // ---- the kernel ----------------------------------------------------------------------------
-template <int kCtas, int kKind, int kAct, int kBits, int kProblems>
-__global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas>::kThreads, 1)
+template <int kCtas, int kKind, int kAct, int kBits, int kProblems, bool kSums = false>
+__global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas, kSums>::kThreads, 1)
     gemm_kernel(const __grid_constant__ GemmParams<kProblems> g) {
-  using L = GemmLayout<kKind, kBits, kCtas>;
+  using L = GemmLayout<kKind, kBits, kCtas, kSums>;
   constexpr int kStages = L::kStages;
   constexpr bool kPair = kCtas == 2;
   extern __shared__ uint8_t smem_raw[];
@@ -469,7 +477,9 @@ __global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas>::kThreads, 1)
     // A warp works by itself on its 32 rows (its lane is the row) and on every other 64 columns, or on one piece of 32 columns
     // in three; it waits for no other warp. 12 warps instead of 8 for the epilogues with much to compute: a warp's own latencies
     // (tensor memory, exponentials, code blocks) left three quarters of the issue slots empty. Their rows go out as whole
-    // sectors from registers. (Boxes for TMA instead cost a proxy fence and shared memory, which is the stages'.)
+    // sectors from registers; boxes for TMA take shared memory that the stages need (131072 x 512 x 1368 in 8 bits: 408
+    // instead of 372 us). With column sums (kSums) it is the other way round: their shuffles queue behind the plain stores
+    // (26253 x 768 x 2048 in 8 bits: 156, with boxes 123).
     const int wg = (warp >> 2) - 1, quarter = warp & 3;
     [[maybe_unused]] const uint32_t own = base + L::kWarps + (warp - 4) * L::kWarpBytes;
     const uint32_t lanes = uint32_t(quarter) << 21;
@@ -503,7 +513,7 @@ __global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas>::kThreads, 1)
         }
         if (ahead.live && lane == 0) {
           mbar_arrive_expect_tx(my_codes + 8 * slot, Block::kBytes);
-          bulk_load(own + slot * Block::kBytes, code_block(ahead.u, ahead.u.col * cols + ahead.blk), Block::kBytes,
+          bulk_load(own + L::kBoxes + slot * Block::kBytes, code_block(ahead.u, ahead.u.col * cols + ahead.blk), Block::kBytes,
                     my_codes + 8 * slot);
         }
       }
@@ -560,12 +570,12 @@ __global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas>::kThreads, 1)
           }
         }
       } else if constexpr (kKind == kGemmDact) {
-        const int64_t at_row = int64_t(row + lane) * g.stride;
+        [[maybe_unused]] const int64_t at_row = int64_t(row + lane) * g.stride;
 #pragma unroll 1
         for (int blk = first_piece(i, p.cols / 32); blk < p.cols; blk += 32 * L::kTeams) {
           const int f = u.col * p.cols + blk;
           if (f >= g.hidden) break;
-          const uint32_t slot = piece % L::kSlots, codes = own + slot * Block::kBytes;
+          const uint32_t slot = piece % L::kSlots, codes = own + L::kBoxes + slot * Block::kBytes;
           mbar_wait(my_codes + 8 * slot, (piece / L::kSlots) & 1, abort_flag);
           uint32_t scales;
           asm volatile("ld.shared.b32 %0, [%1];" : "=r"(scales) : "r"(codes + Block::kScales + lane * 4) : "memory");
@@ -606,12 +616,30 @@ __global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas>::kThreads, 1)
               }
             }
             const int fq = f + 16 * q;
-            if (row + lane < p.m && fq < g.hidden) {
+            if constexpr (kSums) {
+              if (q == 0) {
+                if (lane == 0) bulk_wait_group_read0();  // the boxes in front have left
+                __syncwarp();
+              }
+              stage_half16(own, lane, q, vd);
+              stage_half16(own + 2048, lane, q, ve);
+              if constexpr (kBits == 8) stage_half16(own + 4096, lane, q, vh);
+              if (q == 1) {
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                  tma_store_2d(&p.c, own, f, row);
+                  tma_store_2d(&g.map_db, own + 2048, f, row);
+                  if constexpr (kBits == 8) tma_store_2d(&g.map_h, own + 4096, f, row);
+                  bulk_commit_group();
+                }
+              }
+            } else if (row + lane < p.m && fq < g.hidden) {
               store_sector(g.da + at_row + fq, vd);
               store_sector(g.db + at_row + fq, ve);
               if constexpr (kBits == 8) store_sector(g.h + at_row + fq, vh);
             }
-            if (g.col_sums != nullptr) {
+            if constexpr (kSums) {
               float* sums = g.col_sums + (int64_t(row0 / kGemmRows) * 4 + quarter) * (2 * int64_t(g.hidden));
               const float sd = column_sums(d, lane), se = column_sums(e, lane);
               const int at = fq + (lane & 15);
