@@ -251,12 +251,12 @@ int launch(void (*kernel)(Arg), dim3 grid, unsigned threads, size_t smem, void* 
 
 // A GEMM kernel needs its shared memory allowed once per device.
 constexpr int kMaxDevices = 64;
-template <int kCtas, int kKind, int kAct, int kBits, int kProblems, bool kSums>
-int launch_team(const GemmParams<kProblems>& g, int sms, void* stream) {
+template <int kCtas, int kKind, int kAct, int kBits, int kProblems>
+int launch_gemm(const GemmParams<kProblems>& g, int sms, void* stream) {
   static std::mutex mutex;
   static bool ready[kMaxDevices];
-  auto* kernel = gemm_kernel<kCtas, kKind, kAct, kBits, kProblems, kSums>;
-  using L = GemmLayout<kKind, kBits, kCtas, kSums>;
+  auto* kernel = gemm_kernel<kCtas, kKind, kAct, kBits, kProblems>;
+  using L = GemmLayout<kKind, kBits, kCtas>;
   constexpr int kSmem = L::kBytes;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return NB_ATTN_ERR_DEVICE;
@@ -269,14 +269,12 @@ int launch_team(const GemmParams<kProblems>& g, int sms, void* stream) {
     }
   }
   const int units = g.deal.n_long + g.deal.n_short, teams = std::min(units, sms / kCtas);
-  return launch(kernel, dim3(unsigned(teams * kCtas)), L::kThreads, kSmem, stream, g, kCtas);
+  return launch(kernel, dim3(unsigned(teams * kCtas)), kGemmThreads, kSmem, stream, g, kCtas);
 }
-template <int kKind, int kAct, int kBits, int kProblems, bool kSums = false>
+template <int kKind, int kAct, int kBits, int kProblems>
 int launch_gemm(const GemmParams<kProblems>& g, int ctas, int sms, void* stream) {
-  if constexpr (kKind == kGemmDact && !kSums)
-    if (g.col_sums != nullptr) return launch_gemm<kKind, kAct, kBits, kProblems, true>(g, ctas, sms, stream);
-  return ctas == 2 ? launch_team<2, kKind, kAct, kBits, kProblems, kSums>(g, sms, stream)
-                   : launch_team<1, kKind, kAct, kBits, kProblems, kSums>(g, sms, stream);
+  return ctas == 2 ? launch_gemm<2, kKind, kAct, kBits, kProblems>(g, sms, stream)
+                   : launch_gemm<1, kKind, kAct, kBits, kProblems>(g, sms, stream);
 }
 
 int div_up(int64_t a, int64_t b) { return int((a + b - 1) / b); }
@@ -491,8 +489,6 @@ extern "C" int nb_gated_mlp_fwd(const nb_gated_mlp_fwd_args* args, void* stream)
   NB_TRY(check_matrix(args->w_down, s.hidden));
   NB_TRY(check_matrix(args->y, s.dim));
   NB_TRY(check_matrix(args->h, s.hidden));
-  // (16 values at a time are written there)
-  if ((reinterpret_cast<uintptr_t>(args->h.ptr) & 31u) != 0 || args->h.stride % 16 != 0) return NB_ATTN_ERR_ALIGN;
   for (const void* b : {args->b_gate, args->b_up, args->b_down}) NB_TRY(check_bias(b));
   if (s.checkpoint != NB_CHECKPOINT_NONE) {
     if (args->checkpoint == nullptr) return NB_ATTN_ERR_NULL;
@@ -514,7 +510,7 @@ extern "C" int nb_gated_mlp_fwd(const nb_gated_mlp_fwd_args* args, void* stream)
   NB_TRY(map_k_major(&p.a[0], args->x, s.tokens, s.dim, kGemmRows));
   NB_TRY(map_k_major(&p.b[0], args->w_gate, s.hidden, s.dim, cols / 2));
   NB_TRY(map_k_major(&p.b[1], args->w_up, s.hidden, s.dim, cols / 2));
-  g.h = static_cast<bf16*>(args->h.ptr), g.stride = args->h.stride;
+  NB_TRY(host_matrix_map(&p.c, args->h.ptr, s.tokens, s.hidden, args->h.stride, 32, kGroup));
   p.bias = static_cast<const bf16*>(args->b_gate);
   g.bias_up = static_cast<const bf16*>(args->b_up);
   g.codes = static_cast<uint8_t*>(args->checkpoint);
@@ -588,14 +584,11 @@ extern "C" int nb_gated_mlp_bwd(const nb_gated_mlp_bwd_args* args, void* stream)
     p.b_mn = 1;
     NB_TRY(map_k_major(&p.a[0], a.dy, s.tokens, s.dim, kGemmRows));
     NB_TRY(map_mn_major(&p.b[0], a.w_down, s.dim, s.hidden));
-    g.da = static_cast<bf16*>(da.ptr), g.db = static_cast<bf16*>(db.ptr), g.h = static_cast<bf16*>(h.ptr), g.stride = da.stride;
-    if (a.d_b_gate != nullptr || a.d_b_up != nullptr) {
-      g.col_sums = reinterpret_cast<float*>(ws + plan.col_sums);
-      NB_TRY(host_matrix_map(&p.c, da.ptr, s.tokens, s.hidden, da.stride, 32, kGroup));
-      NB_TRY(host_matrix_map(&g.map_db, db.ptr, s.tokens, s.hidden, db.stride, 32, kGroup));
-      if (s.checkpoint == NB_CHECKPOINT_8BIT)
-        NB_TRY(host_matrix_map(&g.map_h, h.ptr, s.tokens, s.hidden, h.stride, 32, kGroup));
-    }
+    NB_TRY(host_matrix_map(&p.c, da.ptr, s.tokens, s.hidden, da.stride, 32, kGroup));
+    NB_TRY(host_matrix_map(&g.map_db, db.ptr, s.tokens, s.hidden, db.stride, 32, kGroup));
+    if (s.checkpoint == NB_CHECKPOINT_8BIT)
+      NB_TRY(host_matrix_map(&g.map_h, h.ptr, s.tokens, s.hidden, h.stride, 32, kGroup));
+    if (a.d_b_gate != nullptr || a.d_b_up != nullptr) g.col_sums = reinterpret_cast<float*>(ws + plan.col_sums);
     g.codes = static_cast<uint8_t*>(const_cast<void*>(a.checkpoint));
     g.groups = div_up(s.hidden, kGroup), g.hidden = s.hidden;
     g.deal.n_short = p.row_tiles * p.col_tiles;

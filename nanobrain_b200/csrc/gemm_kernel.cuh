@@ -38,15 +38,13 @@ struct CodeBlock {
 };
 
 // Shared memory: stages, then a part for every epilogue warp (boxes for TMA's stores, code blocks), then barriers.
-template <int kKind, int kBits, int kCtas, bool kSums>
+constexpr int kEpilogueWarps = 8, kGemmThreads = 128 + 32 * kEpilogueWarps;
+template <int kKind, int kBits, int kCtas>
 struct GemmLayout {
-  static constexpr int kTeams = kKind == kGemmPlain ? 2 : 3;  // of four warps, for the 128 rows of a tile
-  static constexpr int kEpilogueWarps = 4 * kTeams;
-  static constexpr int kThreads = 128 + 32 * kEpilogueWarps;
   static constexpr int kStageBytes = kGemmBytesA + kGemmBytesB / kCtas;
-  static constexpr int kSlots = kKind != kGemmDact ? 0 : kBits == 8 && !kSums ? 2 : 1;  // code blocks under way
-  static constexpr int kBoxes = kKind == kGemmPlain ? 4096 : kKind == kGemmDact && kSums ? (kBits == 8 ? 3 : 2) * 2048 : 0;
-  static constexpr int kWarpBytes = (kBoxes + kSlots * CodeBlock<kBits>::kBytes + 511) / 512 * 512;
+  static constexpr int kBoxes = kKind == kGemmPlain ? 4096 : kKind == kGemmGate ? 2048 : (kBits == 8 ? 3 : 2) * 2048;
+  static constexpr int kSlots = kKind == kGemmDact && kBits == 8 ? 2 : 1;  // code blocks under way
+  static constexpr int kWarpBytes = (kBoxes + kSlots * CodeBlock<kBits>::kBytes + 1023) / 1024 * 1024;
   static constexpr int kMost = 232448 - 1024 - 512 - kEpilogueWarps * kWarpBytes;
   static constexpr int kStages = kMost / kStageBytes < 6 ? kMost / kStageBytes : 6;
   static constexpr int kWarps = kStages * kStageBytes;
@@ -103,12 +101,10 @@ struct GemmParams {
   GemmDeal deal;
   int32_t* status;
   // the gate's and its backward's
-  CUtensorMap map_db, map_h;   // backward with kSums: and p[0].c of da
-  __nv_bfloat16 *da, *db, *h;  // rows of `stride` values, at 32 bytes
-  int64_t stride;
+  CUtensorMap map_db, map_h;   // backward (p[0].c is that of da, forward of h)
   const __nv_bfloat16* bias_up;
   uint8_t* codes;     // checkpoint: [row tile][group][warp] code blocks
-  float* col_sums;    // backward with kSums: [row tile][warp][2 x hidden] sums of da and db over 32 rows
+  float* col_sums;    // backward, or NULL: [row tile][warp][2 x hidden] sums of da and db over 32 rows
   int32_t groups, hidden;
 };
 
@@ -334,12 +330,6 @@ __device__ __forceinline__ void stage_half16(uint32_t box, int row, int half, co
   for (int i = 0; i < 2; ++i)
     st_shared_v4(box + row * 64 + (((2 * half + i) ^ ((row >> 1) & 3)) << 4), w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
 }
-// 16 values to 32 bytes (a whole sector) of a row.
-__device__ __forceinline__ void store_sector(__nv_bfloat16* p, const uint32_t (&w)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
-               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-               : "memory");
-}
 __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
@@ -347,26 +337,25 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
 }
 
 // ---- the kernel ----------------------------------------------------------------------------
-template <int kCtas, int kKind, int kAct, int kBits, int kProblems, bool kSums = false>
-__global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas, kSums>::kThreads, 1)
-    gemm_kernel(const __grid_constant__ GemmParams<kProblems> g) {
-  using L = GemmLayout<kKind, kBits, kCtas, kSums>;
+template <int kCtas, int kKind, int kAct, int kBits, int kProblems>
+__global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmParams<kProblems> g) {
+  using L = GemmLayout<kKind, kBits, kCtas>;
   constexpr int kStages = L::kStages;
   constexpr bool kPair = kCtas == 2;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t bars = base + L::kBars;
   const uint32_t full = bars, empty = bars + 8 * kStages, acc_full = bars + 16 * kStages, acc_empty = acc_full + 16,
-                 codes_full = acc_empty + 16, tmem_slot = codes_full + 16 * L::kEpilogueWarps, abort_at = tmem_slot + 4;
+                 codes_full = acc_empty + 16, tmem_slot = codes_full + 16 * kEpilogueWarps, abort_at = tmem_slot + 4;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_raw + (abort_at - smem_u32(smem_raw)));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = kPair ? int(cluster_rank()) : 0;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
-    for (int i = 0; i < 2; ++i) mbar_init(acc_full + 8 * i, 1), mbar_init(acc_empty + 8 * i, L::kEpilogueWarps * kCtas);
+    for (int i = 0; i < 2; ++i) mbar_init(acc_full + 8 * i, 1), mbar_init(acc_empty + 8 * i, kEpilogueWarps * kCtas);
     if constexpr (kKind == kGemmDact)
-      for (int i = 0; i < 2 * L::kEpilogueWarps; ++i) mbar_init(codes_full + 8 * i, 1);
+      for (int i = 0; i < 2 * kEpilogueWarps; ++i) mbar_init(codes_full + 8 * i, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -474,23 +463,17 @@ __global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas, kSums>::kThrea
       }
     }
   } else if (warp >= 4) {
-    // A warp works by itself on its 32 rows (its lane is the row) and on every other 64 columns, or on one piece of 32 columns
-    // in three; it waits for no other warp. 12 warps instead of 8 for the epilogues with much to compute: a warp's own latencies
-    // (tensor memory, exponentials, code blocks) left three quarters of the issue slots empty. Their rows go out as whole
-    // sectors from registers; boxes for TMA take shared memory that the stages need (131072 x 512 x 1368 in 8 bits: 408
-    // instead of 372 us). With column sums (kSums) it is the other way round: their shuffles queue behind the plain stores
-    // (26253 x 768 x 2048 in 8 bits: 156, with boxes 123).
+    // A warp works by itself on its 32 rows (its lane is the row) and on every other 32 (plain: 64) columns, hands boxes of 32
+    // rows to TMA and waits for no other warp. (Four warps that met at two barriers per box spent 17 % of their time there.)
+    // Twelve warps that store whole sectors from their registers instead save 5 of 125 us in the gate with 16 bits and no
+    // biases (26253 x 768 x 2048), but what else uses the load and store unit queues behind such stores: with biases
+    // the gate took 130 instead of 108 us in 8 bits, the activation's backward with its column sums 155 instead of 118.
     const int wg = (warp >> 2) - 1, quarter = warp & 3;
     [[maybe_unused]] const uint32_t own = base + L::kWarps + (warp - 4) * L::kWarpBytes;
     const uint32_t lanes = uint32_t(quarter) << 21;
     const uint32_t acc_free = kPair ? map_to_rank(acc_empty, 0) : acc_empty;  // where the MMAs' issuer waits
     constexpr int kB = kBits ? kBits : 16;
     using Block = CodeBlock<kB>;
-    // The first column of this warp's pieces in the CTA's i-th unit: pieces are dealt out across the units.
-    [[maybe_unused]] const auto first_piece = [&](int i, int pieces) {
-      const int at = (wg - i * pieces) % L::kTeams;
-      return (at < 0 ? at + L::kTeams : at) * 32;
-    };
     const auto rows_of = [&](const GemmUnit& u) { return (u.row * kCtas + rank) * kGemmRows; };
     const auto code_block = [&](const GemmUnit& u, int f) {
       return g.codes + ((int64_t(u.row * kCtas + rank) * g.groups + f / kGroup) * 4 + quarter) * Block::kBytes;
@@ -503,13 +486,13 @@ __global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas, kSums>::kThrea
     [[maybe_unused]] const auto request = [&](uint32_t slot) {  // the next piece's
       if constexpr (kKind == kGemmDact) {
         const int cols = g.p[0].cols;
-        ahead.blk += 32 * L::kTeams;
+        ahead.blk += 64;
         while (ahead.live && (ahead.i < 0 || ahead.blk >= cols || ahead.u.col * cols + ahead.blk >= g.hidden ||
                               (kPair && rows_of(ahead.u) >= g.p[0].m))) {
           const int id = turns.unit(++ahead.i);
           ahead.live = id >= 0;
           if (ahead.live) ahead.u = gemm_unit(g, id);
-          ahead.blk = first_piece(ahead.i, cols / 32);
+          ahead.blk = wg * 32;
         }
         if (ahead.live && lane == 0) {
           mbar_arrive_expect_tx(my_codes + 8 * slot, Block::kBytes);
@@ -518,7 +501,8 @@ __global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas, kSums>::kThrea
         }
       }
     };
-    for (int i = 0; i < L::kSlots; ++i) request(i);
+    if constexpr (kKind == kGemmDact)
+      for (int i = 0; i < L::kSlots; ++i) request(i);
 
     for (int i = 0;; ++i) {
       const int id = turns.unit(i);
@@ -533,21 +517,22 @@ __global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas, kSums>::kThrea
         // the pair's second half lies behind the last row
       } else if constexpr (kKind == kGemmGate) {
         const int half = p.cols / 2;
-        __nv_bfloat16* h_row = g.h + int64_t(row + lane) * g.stride;
 #pragma unroll 1
-        for (int blk = first_piece(i, half / 32); blk < half; blk += 32 * L::kTeams) {
+        for (int blk = wg * 32; blk < half; blk += 64) {
           const int f = u.col * half + blk;
           if (f >= g.hidden) break;
-          [[maybe_unused]] uint8_t* block = kBits > 0 ? code_block(u, f) : nullptr;
+          [[maybe_unused]] const uint32_t block = own + L::kBoxes;
           float a[32], b[32];
           [[maybe_unused]] uint32_t w[Block::kWords], scales = 0;
           tmem_ld32f(acc + blk, a);
           add_bias32(a, p.bias, f, g.hidden);
+          if (lane == 0) bulk_wait_group_read0();  // the boxes in front have left
+          __syncwarp();
           if constexpr (kBits > 0) {
             scales = encode<kB>(a, w);
 #pragma unroll
             for (int c = 0; c < Block::kChunks; ++c)
-              *reinterpret_cast<uint4*>(block + c * 512 + lane * 16) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+              st_shared_v4(block + c * 512 + lane * 16, w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
           }
 #pragma unroll
           for (int k = 0; k < 32; k += 2) split(gate_of<kAct>(make_float2(a[k], a[k + 1])), a[k], a[k + 1]);
@@ -557,22 +542,28 @@ __global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas, kSums>::kThrea
             scales |= encode<kB>(b, w) << 16;
 #pragma unroll
             for (int c = 0; c < Block::kChunks; ++c)
-              *reinterpret_cast<uint4*>(block + (Block::kChunks + c) * 512 + lane * 16) =
-                  make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
-            *reinterpret_cast<uint32_t*>(block + Block::kScales + lane * 4) = scales;
+              st_shared_v4(block + (Block::kChunks + c) * 512 + lane * 16, w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(block + Block::kScales + lane * 4), "r"(scales) : "memory");
           }
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             uint32_t v[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = pack_bf16(a[16 * q + 2 * k] * b[16 * q + 2 * k], a[16 * q + 2 * k + 1] * b[16 * q + 2 * k + 1]);
-            if (row + lane < p.m) store_sector(h_row + f + 16 * q, v);  // (the rows' padding takes what is behind `hidden`)
+            for (int k = 0; k < 8; ++k)
+              v[k] = pack_bf16(a[16 * q + 2 * k] * b[16 * q + 2 * k], a[16 * q + 2 * k + 1] * b[16 * q + 2 * k + 1]);
+            stage_half16(own, lane, q, v);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&p.c, own, f, row);
+            if constexpr (kBits > 0) bulk_store(code_block(u, f), block, Block::kBytes);
+            bulk_commit_group();
           }
         }
       } else if constexpr (kKind == kGemmDact) {
-        [[maybe_unused]] const int64_t at_row = int64_t(row + lane) * g.stride;
 #pragma unroll 1
-        for (int blk = first_piece(i, p.cols / 32); blk < p.cols; blk += 32 * L::kTeams) {
+        for (int blk = wg * 32; blk < p.cols; blk += 64) {
           const int f = u.col * p.cols + blk;
           if (f >= g.hidden) break;
           const uint32_t slot = piece % L::kSlots, codes = own + L::kBoxes + slot * Block::kBytes;
@@ -580,29 +571,26 @@ __global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas, kSums>::kThrea
           uint32_t scales;
           asm volatile("ld.shared.b32 %0, [%1];" : "=r"(scales) : "r"(codes + Block::kScales + lane * 4) : "memory");
           const float2 sa = both(__uint_as_float(scales << 16)), sb = both(__uint_as_float(scales & 0xFFFF0000u));
-          constexpr int kHalf = Block::kChunks / 2;  // chunks of 16 values
+          uint32_t wa[Block::kWords], wb[Block::kWords], r[32];
+          tmem_ld32(acc + blk, r);
+#pragma unroll
+          for (int c = 0; c < Block::kChunks; ++c) {
+            const uint4 x = ld_shared_v4(codes + c * 512 + lane * 16),
+                        y = ld_shared_v4(codes + (Block::kChunks + c) * 512 + lane * 16);
+            wa[4 * c] = x.x, wa[4 * c + 1] = x.y, wa[4 * c + 2] = x.z, wa[4 * c + 3] = x.w;
+            wb[4 * c] = y.x, wb[4 * c + 1] = y.y, wb[4 * c + 2] = y.z, wb[4 * c + 3] = y.w;
+          }
+          __syncwarp();
+          request(slot);  // the block has been read
+          tmem_wait_ld();
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            uint32_t wa[4 * kHalf], wb[4 * kHalf], r[16];
-            tmem_ld16(acc + blk + 16 * q, r);
-#pragma unroll
-            for (int c = 0; c < kHalf; ++c) {
-              const uint4 x = ld_shared_v4(codes + (q * kHalf + c) * 512 + lane * 16),
-                          y = ld_shared_v4(codes + (Block::kChunks + q * kHalf + c) * 512 + lane * 16);
-              wa[4 * c] = x.x, wa[4 * c + 1] = x.y, wa[4 * c + 2] = x.z, wa[4 * c + 3] = x.w;
-              wb[4 * c] = y.x, wb[4 * c + 1] = y.y, wb[4 * c + 2] = y.z, wb[4 * c + 3] = y.w;
-            }
-            tmem_wait_ld();
-            if (q == 1) {  // the block has been read
-              __syncwarp();
-              request(slot);
-            }
             float d[16], e[16];
             uint32_t vd[8], ve[8], vh[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              const float2 a = decode<kB>(wa, k, sa), b = decode<kB>(wb, k, sb),
-                             dh = make_float2(__uint_as_float(r[2 * k]), __uint_as_float(r[2 * k + 1]));
+              const float2 a = decode<kB>(wa, 8 * q + k, sa), b = decode<kB>(wb, 8 * q + k, sb),
+                           dh = make_float2(__uint_as_float(r[16 * q + 2 * k]), __uint_as_float(r[16 * q + 2 * k + 1]));
               float2 gate, slope;
               gate_and_slope<kAct>(a, gate, slope);
               split(__fmul2_rn(dh, gate), e[2 * k], e[2 * k + 1]);
@@ -615,31 +603,25 @@ __global__ void __launch_bounds__(GemmLayout<kKind, kBits, kCtas, kSums>::kThrea
                 vh[k] = pack_bf16(x, y);
               }
             }
-            const int fq = f + 16 * q;
-            if constexpr (kSums) {
-              if (q == 0) {
-                if (lane == 0) bulk_wait_group_read0();  // the boxes in front have left
-                __syncwarp();
-              }
-              stage_half16(own, lane, q, vd);
-              stage_half16(own + 2048, lane, q, ve);
-              if constexpr (kBits == 8) stage_half16(own + 4096, lane, q, vh);
-              if (q == 1) {
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                  tma_store_2d(&p.c, own, f, row);
-                  tma_store_2d(&g.map_db, own + 2048, f, row);
-                  if constexpr (kBits == 8) tma_store_2d(&g.map_h, own + 4096, f, row);
-                  bulk_commit_group();
-                }
-              }
-            } else if (row + lane < p.m && fq < g.hidden) {
-              store_sector(g.da + at_row + fq, vd);
-              store_sector(g.db + at_row + fq, ve);
-              if constexpr (kBits == 8) store_sector(g.h + at_row + fq, vh);
+            if (q == 0) {
+              if (lane == 0) bulk_wait_group_read0();  // the boxes in front have left
+              __syncwarp();
             }
-            if constexpr (kSums) {
+            stage_half16(own, lane, q, vd);
+            stage_half16(own + 2048, lane, q, ve);
+            if constexpr (kBits == 8) stage_half16(own + 4096, lane, q, vh);
+            if (q == 1) {
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_2d(&p.c, own, f, row);
+                tma_store_2d(&g.map_db, own + 2048, f, row);
+                if constexpr (kBits == 8) tma_store_2d(&g.map_h, own + 4096, f, row);
+                bulk_commit_group();
+              }
+            }
+            if (g.col_sums != nullptr) {
+              const int fq = f + 16 * q;
               float* sums = g.col_sums + (int64_t(row0 / kGemmRows) * 4 + quarter) * (2 * int64_t(g.hidden));
               const float sd = column_sums(d, lane), se = column_sums(e, lane);
               const int at = fq + (lane & 15);
