@@ -119,7 +119,7 @@ if not globals().get("_flop_formulas"):
 
 def _observed(*tensors) -> bool:
     """Tracing and overrides see the op itself."""
-    return torch.compiler.is_compiling() or has_torch_function(tuple(t for t in tensors if t is not None))
+    return torch.compiler.is_compiling() or has_torch_function(tensors)
 
 
 def qk_norm_rope(
@@ -150,8 +150,8 @@ def qk_norm_rope(
     Every token is treated by itself, rows behind the last sequence of a packed buffer too."""
     if _observed(q, k, q_weight, k_weight, positions, k_positions, freqs):
         return qk_norm_rope_fwd(q, k, q_weight, k_weight, positions, k_positions, freqs, float(eps), bool(interleaved))
-    return ops._load_native().qk_norm_rope(q, k, q_weight, k_weight, positions, k_positions, freqs, float(eps),
-                                           bool(interleaved))
+    native = ops._native or ops._load_native()
+    return native.qk_norm_rope(q, k, q_weight, k_weight, positions, k_positions, freqs, float(eps), bool(interleaved))
 
 
 def gated_mlp(
@@ -189,4 +189,4 @@ def gated_mlp(
         if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args)):
             codes = codes[0], 0  # nothing goes back: nothing is kept
         return gated_mlp_fwd(*args, *codes)[0]
-    return ops._load_native().gated_mlp(*args, *codes)
+    return (ops._native or ops._load_native()).gated_mlp(*args, *codes)

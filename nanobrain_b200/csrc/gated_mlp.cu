@@ -161,6 +161,7 @@ __global__ void __launch_bounds__(256) split_sum_kernel(const __grid_constant__ 
 
 // Sums of a matrix' columns over chunks of kSumRows rows: a block takes 64 columns.
 constexpr int kSumRows = 512;
+constexpr int kDirectRows = 4096;  // up to so many rows the last kernel reads the matrix itself: a launch less
 struct ColPartialParams {
   const bf16* m;
   int64_t stride, rows;
@@ -199,10 +200,11 @@ __global__ void __launch_bounds__(256) col_partial_kernel(const __grid_constant_
 }
 
 struct ColItem {
-  const float* partial;  // [rows][stride]
+  const void* from;      // fp32 or bf16 [rows][stride]
   bf16* out;
   int64_t stride;
   int32_t rows, n, blocks;
+  int32_t is_bf16;
 };
 struct ColParams {
   ColItem item[3];
@@ -218,8 +220,13 @@ __global__ void __launch_bounds__(1024) col_sum_kernel(const __grid_constant__ C
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = b * 32 + lane;
   float v = 0.f;
   if (c < s.n) {
+    if (s.is_bf16) {
 #pragma unroll 8
-    for (int r = warp; r < s.rows; r += 32) v += s.partial[r * s.stride + c];
+      for (int r = warp; r < s.rows; r += 32) v += __bfloat162float(static_cast<const bf16*>(s.from)[r * s.stride + c]);
+    } else {
+#pragma unroll 8
+      for (int r = warp; r < s.rows; r += 32) v += static_cast<const float*>(s.from)[r * s.stride + c];
+    }
   }
   part[warp][lane] = v;
   __syncthreads();
@@ -232,8 +239,9 @@ __global__ void __launch_bounds__(1024) col_sum_kernel(const __grid_constant__ C
 }
 
 // ---- host --------------------------------------------------------------------------------------
-template <typename Arg>
-int launch(void (*kernel)(Arg), dim3 grid, unsigned threads, size_t smem, void* stream, const Arg& arg, int cluster = 1) {
+template <typename... KArgs>
+int launch_cluster(void (*kernel)(KArgs...), int cluster, dim3 grid, unsigned threads, size_t smem, void* stream,
+                   const KArgs&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -246,7 +254,11 @@ int launch(void (*kernel)(Arg), dim3 grid, unsigned threads, size_t smem, void* 
   attr[1].val.clusterDim.x = unsigned(cluster), attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, arg) == cudaSuccess ? NB_ATTN_OK : NB_ATTN_ERR_LAUNCH;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? NB_ATTN_OK : NB_ATTN_ERR_LAUNCH;
+}
+template <typename Arg>
+int launch(void (*kernel)(Arg), dim3 grid, unsigned threads, size_t smem, void* stream, const Arg& arg) {
+  return launch_cluster(kernel, 1, grid, threads, smem, stream, arg);
 }
 
 // A GEMM kernel needs its shared memory allowed once per device.
@@ -269,7 +281,7 @@ int launch_gemm(const GemmParams<kProblems>& g, int sms, void* stream) {
     }
   }
   const int units = g.deal.n_long + g.deal.n_short, teams = std::min(units, sms / kCtas);
-  return launch(kernel, dim3(unsigned(teams * kCtas)), kGemmThreads, kSmem, stream, g, kCtas);
+  return launch_cluster(kernel, kCtas, dim3(unsigned(teams * kCtas)), kGemmThreads, kSmem, stream, g, GemmTail{g.status, {}});
 }
 template <int kKind, int kAct, int kBits, int kProblems>
 int launch_gemm(const GemmParams<kProblems>& g, int ctas, int sms, void* stream) {
@@ -462,7 +474,7 @@ BwdPlan plan_bwd(const nb_gated_mlp_bwd_args& a, int sms) {
   p.h = take(s.checkpoint == NB_CHECKPOINT_8BIT ? hidden_bytes : 0);
   const size_t row_tiles = size_t(div_up(s.tokens, kGemmRows));
   p.col_sums = take(a.d_b_gate != nullptr || a.d_b_up != nullptr ? row_tiles * 4 * 2 * s.hidden * 4 : 0);
-  p.dy_sums = take(a.d_b_down != nullptr ? size_t(div_up(s.tokens, kSumRows)) * s.dim * 4 : 0);
+  p.dy_sums = take(a.d_b_down != nullptr && s.tokens > kDirectRows ? size_t(div_up(s.tokens, kSumRows)) * s.dim * 4 : 0);
   // All products of the launch have teams of one size.
   BwdPlan best = plan_products(p, a, sms, 2);
   const BwdPlan single = plan_products(p, a, sms, 1);
@@ -662,19 +674,21 @@ extern "C" int nb_gated_mlp_bwd(const nb_gated_mlp_bwd_args* args, void* stream)
 
   // Biases.
   ColParams cols{};
-  const auto add_col = [&](void* out, const float* partial, int64_t stride, int rows, int width) {
+  const auto add_col = [&](void* out, const void* from, bool is_bf16, int64_t stride, int rows, int width) {
     if (out == nullptr) return;
-    cols.item[cols.n_items++] = ColItem{partial, static_cast<bf16*>(out), stride, rows, width, div_up(width, 32)};
+    cols.item[cols.n_items++] = ColItem{from, static_cast<bf16*>(out), stride, rows, width, div_up(width, 32), is_bf16};
   };
   const float* sums_at = reinterpret_cast<const float*>(ws + plan.col_sums);
-  add_col(a.d_b_gate, sums_at, 2 * int64_t(s.hidden), row_tiles * 4, s.hidden);
-  add_col(a.d_b_up, sums_at + s.hidden, 2 * int64_t(s.hidden), row_tiles * 4, s.hidden);
-  if (a.d_b_down != nullptr) {
+  add_col(a.d_b_gate, sums_at, false, 2 * int64_t(s.hidden), row_tiles * 4, s.hidden);
+  add_col(a.d_b_up, sums_at + s.hidden, false, 2 * int64_t(s.hidden), row_tiles * 4, s.hidden);
+  if (s.tokens <= kDirectRows) {
+    add_col(a.d_b_down, a.dy.ptr, true, a.dy.stride, int(s.tokens), s.dim);
+  } else if (a.d_b_down != nullptr) {
     float* dy_sums = reinterpret_cast<float*>(ws + plan.dy_sums);
     const int chunks = div_up(s.tokens, kSumRows);
     NB_TRY(launch(col_partial_kernel, dim3(div_up(s.dim, 64), chunks), 256, 0, stream,
                   ColPartialParams{static_cast<const bf16*>(a.dy.ptr), a.dy.stride, s.tokens, dy_sums, s.dim}));
-    add_col(a.d_b_down, dy_sums, s.dim, chunks, s.dim);
+    add_col(a.d_b_down, dy_sums, false, s.dim, chunks, s.dim);
   }
   if (cols.n_items > 0) {
     int blocks = 0;

@@ -60,7 +60,7 @@ void check_heads(const Tensor& t, const char* name) {
 
 struct QkCall {
   nb_qk_norm_rope_args args{};
-  std::vector<Tensor> keep;  // what the arguments point into
+  std::vector<Tensor> keep;  // copies that the arguments point into
 };
 
 nb_attn_tensor desc_of(const Tensor& t) { return t.dim() == 4 ? nbt::dense_desc(t) : nbt::packed_desc(t); }
@@ -89,8 +89,9 @@ void set_side(QkCall& c, nb_qk_side& s, const Tensor& x, const MaybeTensor& weig
                weight_name, " must be [64] on the device of q");
     QK_REQUIRE(weight->scalar_type() == at::kFloat || weight->scalar_type() == at::kBFloat16, weight_name,
                " must be float32 or bfloat16, got ", weight->scalar_type());
-    c.keep.push_back(weight->to(at::kFloat).contiguous());
-    s.weight = c.keep.back().data_ptr<float>();
+    const bool as_is = weight->scalar_type() == at::kFloat && weight->stride(0) == 1;
+    if (!as_is) c.keep.push_back(weight->to(at::kFloat).contiguous());
+    s.weight = (as_is ? *weight : c.keep.back()).data_ptr<float>();
   }
   if (c.args.axes == 0) return;
   QK_REQUIRE(has(positions), positions_name, " are missing");
@@ -106,8 +107,9 @@ void set_side(QkCall& c, nb_qk_side& s, const Tensor& x, const MaybeTensor& weig
   QK_REQUIRE(type >= 0, positions_name, " must be int32, int64 or float32, got ", p.scalar_type());
   QK_REQUIRE(c.args.position_type < 0 || c.args.position_type == type, "positions and k_positions must have one type");
   c.args.position_type = type;
-  const Tensor at = p.size(-1) == 1 || p.stride(-1) == 1 ? p : p.contiguous();
-  c.keep.push_back(at);
+  const bool as_is = p.size(-1) == 1 || p.stride(-1) == 1;
+  if (!as_is) c.keep.push_back(p.contiguous());
+  const Tensor& at = as_is ? p : c.keep.back();
   s.positions = at.data_ptr();
   s.position_stride_batch = at.dim() == 3 ? at.stride(0) : 0;
   s.position_stride_token = at.stride(-2);
@@ -129,8 +131,9 @@ QkCall make_call(const Tensor& q, const Tensor& k, const MaybeTensor& q_weight, 
                    freqs->size(1) == kHeadDim / 2 && freqs->size(0) >= 1 && freqs->size(0) <= NB_ROPE_MAX_AXES,
                "freqs must be float32 [axes, 32] with 1 to ", NB_ROPE_MAX_AXES, " axes on the device of q");
     c.args.axes = int32_t(freqs->size(0));
-    c.keep.push_back(freqs->contiguous());
-    c.args.freqs = c.keep.back().data_ptr<float>();
+    const bool as_is = freqs->is_contiguous();
+    if (!as_is) c.keep.push_back(freqs->contiguous());
+    c.args.freqs = (as_is ? *freqs : c.keep.back()).data_ptr<float>();
   }
   set_side(c, c.args.q, q, q_weight, "q_weight", positions, "positions");
   const bool own = has(k_positions);
@@ -203,7 +206,10 @@ struct QkFunction : public torch::autograd::Function<QkFunction> {
         grads[0].defined() ? grads[0] : at::zeros_like(s[0]), grads[1].defined() ? grads[1] : at::zeros_like(s[1]), s[0],
         s[1], maybe(s[2]), maybe(s[3]), maybe(s[4]), maybe(s[5]), maybe(s[6]), ctx->saved_data["eps"].toDouble(),
         ctx->saved_data["interleaved"].toBool());
-    const auto weight_grad = [](const Tensor& g, const Tensor& w) { return w.defined() ? g.to(w.scalar_type()) : Tensor(); };
+    const auto weight_grad = [](const Tensor& g, const Tensor& w) {
+      if (!w.defined()) return Tensor();
+      return w.scalar_type() == at::kFloat ? g : g.to(w.scalar_type());
+    };
     return {dq, dk, weight_grad(dqw, s[2]), weight_grad(dkw, s[3]), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
@@ -382,16 +388,17 @@ struct MlpFunction : public torch::autograd::Function<MlpFunction> {
     ctx->save_for_backward({x, w_gate, w_up, w_down, h, codes});
     ctx->saved_data["activation"] = activation;
     ctx->saved_data["checkpoint"] = checkpoint;
-    std::vector<bool> mask(wanted.begin(), wanted.end());
-    ctx->saved_data["wanted"] = c10::IValue(c10::List<bool>({mask[0], mask[1], mask[2], mask[3], mask[4], mask[5], mask[6]}));
+    int64_t mask = 0;
+    for (size_t i = 0; i < 7; ++i) mask |= int64_t(wanted[i]) << i;
+    ctx->saved_data["wanted"] = mask;
     return {y, h, codes};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return variable_list(9);
     const variable_list s = ctx->get_saved_variables();
-    const auto mask = ctx->saved_data["wanted"].toBoolList();
+    const int64_t mask = ctx->saved_data["wanted"].toInt();
     std::array<bool, 7> wanted;
-    for (size_t i = 0; i < 7; ++i) wanted[i] = mask.get(i);
+    for (size_t i = 0; i < 7; ++i) wanted[i] = (mask >> i) & 1;
     auto [dx, dwg, dwu, dwd, dbg, dbu, dbd] =
         mlp_bwd_op().call(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["activation"].toInt(),
                           ctx->saved_data["checkpoint"].toInt(), wanted);
