@@ -129,7 +129,7 @@ struct SplitItem {
   int64_t pieces;  // of 8 columns x 1 row, over whole tiles
 };
 struct SplitParams {
-  SplitItem item[3];
+  SplitItem item[4];
   int32_t n_items;
 };
 __global__ void __launch_bounds__(256) split_sum_kernel(const __grid_constant__ SplitParams p) {
@@ -416,72 +416,81 @@ void set_tiles(GemmProblem* p, int64_t rows, int n, const Tiling& t, int steps0,
   p->splits = 1, p->split_steps = steps;
 }
 
-// Where the backward's scratch lies in the workspace, and how the products behind it are cut.
+// A product behind da and db: [m][n] over `steps` 64-deep steps, in tiles and parts of the steps.
+enum { kDWGate = 0, kDWUp = 1, kDWDown = 2, kDx = 3, kProducts = 4 };
+struct Product {
+  bool wanted;
+  int64_t m;
+  int n, steps;
+  Tiling tiles;
+  int splits, split_steps;
+  size_t part_bytes;  // fp32 sums of the parts, where there are several
+  double unit_clocks() const { return step_clocks(tiles) * split_steps; }
+  double clocks() const { return step_clocks(tiles) * steps * tiles.row_tiles * tiles.col_tiles; }
+  int units() const { return tiles.row_tiles * tiles.col_tiles * splits; }
+};
+// Where the backward's scratch lies in the workspace, and how its products are cut.
 struct BwdPlan {
-  size_t da, db, h, col_sums, dy_sums, parts[3], bytes;
-  Tiling dx, dw[3];                // dw: of Wg, Wu, Wd
-  int splits[3], split_steps[3];
+  size_t da, db, h, col_sums, dy_sums, parts[kProducts], bytes;
+  int ctas;
+  Product p[kProducts];
   double clocks;
 };
 
-// The products behind da and db by teams of `ctas`; parts[] receives the bytes that are needed there.
-BwdPlan plan_products(BwdPlan p, const nb_gated_mlp_bwd_args& a, int sms, int ctas) {
+// The products by teams of `ctas`.
+void plan_products(BwdPlan* plan, const nb_gated_mlp_bwd_args& a, int sms, int ctas) {
   const nb_gated_mlp_shape& s = a.shape;
-  const int dx_steps = 2 * div_up(s.hidden, kGemmDepth), dw_steps = div_up(s.tokens, kGemmDepth);
-  const bool wanted[3] = {a.d_w_gate.ptr != nullptr, a.d_w_up.ptr != nullptr, a.d_w_down.ptr != nullptr};
-  const auto width = [](int n) { return div_up(div_up(n, div_up(n, kGemmMaxCols)), 64) * 64; };
-  p.dx = tiling(s.tokens, s.dim, dx_steps, sms, ctas, width(s.dim), kPlainClocks);
-  double total = 0.0, longest = 0.0;
-  if (a.dx.ptr != nullptr) {
-    longest = step_clocks(p.dx) * dx_steps;
-    total = longest * p.dx.row_tiles * p.dx.col_tiles;
+  const int tokens = div_up(s.tokens, kGemmDepth), hidden = div_up(s.hidden, kGemmDepth);
+  plan->ctas = ctas;
+  plan->p[kDWGate] = {a.d_w_gate.ptr != nullptr, s.hidden, s.dim, tokens};
+  plan->p[kDWUp] = {a.d_w_up.ptr != nullptr, s.hidden, s.dim, tokens};
+  plan->p[kDWDown] = {a.d_w_down.ptr != nullptr, s.dim, s.hidden, tokens};
+  plan->p[kDx] = {a.dx.ptr != nullptr, s.tokens, s.dim, 2 * hidden};
+  double total = 0.0;
+  for (Product& p : plan->p) {
+    const int cols = div_up(div_up(p.n, div_up(p.n, kGemmMaxCols)), 64) * 64;
+    p.tiles = tiling(p.m, p.n, p.steps, sms, ctas, cols, kPlainClocks);
+    if (p.wanted) total += p.clocks();
   }
-  for (int i = 0; i < 3; ++i) {
-    const int m = i < 2 ? s.hidden : s.dim, n = i < 2 ? s.dim : s.hidden;
-    p.dw[i] = tiling(m, n, dw_steps, sms, ctas, width(n), kPlainClocks);
-    if (wanted[i]) total += step_clocks(p.dw[i]) * p.dw[i].row_tiles * p.dw[i].col_tiles * dw_steps;
-  }
-  // A weight gradient's unit runs over all tokens. Where that is more than a team's even share of the launch's work, it is
-  // cut into parts of about half a share, which are added up behind (fp32, in a fixed order).
+  // A unit that runs over all steps may be more than a team's even share of the launch's work. Then it is cut into parts of
+  // about half a share, which are added up by another launch (fp32, in a fixed order): worth while from some 12000 clocks
+  // on, with parts of 6000 at the least. (26253 x 768 x 2048: nothing is cut; 820 tokens of it: dx, 35 -> 25 us with the sum.)
   const double share = total / (sms / ctas);
-  for (int i = 0; i < 3; ++i) {
-    const double steps = share / step_clocks(p.dw[i]);
+  double longest = 0.0;
+  for (Product& p : plan->p) {
+    const double unit = step_clocks(p.tiles) * p.steps;
     int splits = 1;
-    if (dw_steps > 0.8 * steps) splits = std::min(div_up(dw_steps, 8), int(dw_steps / std::max(0.5 * steps, 8.0)) + 1);
-    // (and a unit stays far below the time after which a wait gives up)
-    splits = std::max({1, std::min(splits, 32), div_up(dw_steps, 1 << 18)});
-    p.split_steps[i] = div_up(dw_steps, splits);
-    p.splits[i] = div_up(dw_steps, p.split_steps[i]);
-    const size_t tiles = size_t(p.dw[i].row_tiles) * ctas * p.dw[i].col_tiles;
-    p.parts[i] = wanted[i] && p.splits[i] > 1 ? tiles * p.dw[i].cols * kGemmRows * 4 * p.splits[i] : 0;
-    if (wanted[i]) longest = std::max(longest, step_clocks(p.dw[i]) * p.split_steps[i]);
+    if (unit > 0.8 * share && unit > 12000.0) splits = std::min(32, int(unit / std::max(0.5 * share, 6000.0)) + 1);
+    splits = std::max(splits, div_up(p.steps, 1 << 18));  // (a unit stays far below the time after which a wait gives up)
+    p.split_steps = div_up(p.steps, splits);
+    p.splits = div_up(p.steps, p.split_steps);
+    const size_t tiles = size_t(p.tiles.row_tiles) * ctas * p.tiles.col_tiles;
+    p.part_bytes = p.wanted && p.splits > 1 ? tiles * p.tiles.cols * kGemmRows * 4 * p.splits : 0;
+    if (p.wanted) longest = std::max(longest, p.unit_clocks());
   }
-  p.clocks = std::max(share + 0.25 * longest, longest) + 1000.0 * ctas;
-  return p;
+  plan->clocks = std::max(share + 0.25 * longest, longest) + 1000.0 * ctas;
 }
 
 BwdPlan plan_bwd(const nb_gated_mlp_bwd_args& a, int sms) {
   const nb_gated_mlp_shape& s = a.shape;
-  BwdPlan p{};
+  BwdPlan p{}, single{};
+  plan_products(&p, a, sms, 2);  // (all products of the launch have teams of one size)
+  plan_products(&single, a, sms, 1);
+  if (single.clocks < 0.98 * p.clocks) p = single;
   size_t at = 0;
   const auto take = [&at](size_t n) {
     const size_t here = at;
     at += align256(n);
     return here;
   };
-  const size_t hidden_bytes = size_t(s.tokens) * padded(s.hidden) * 2;
+  const size_t hidden_bytes = size_t(s.tokens) * padded(s.hidden) * 2, row_tiles = size_t(div_up(s.tokens, kGemmRows));
   p.da = take(hidden_bytes), p.db = take(hidden_bytes);
   p.h = take(s.checkpoint == NB_CHECKPOINT_8BIT ? hidden_bytes : 0);
-  const size_t row_tiles = size_t(div_up(s.tokens, kGemmRows));
   p.col_sums = take(a.d_b_gate != nullptr || a.d_b_up != nullptr ? row_tiles * 4 * 2 * s.hidden * 4 : 0);
   p.dy_sums = take(a.d_b_down != nullptr && s.tokens > kDirectRows ? size_t(div_up(s.tokens, kSumRows)) * s.dim * 4 : 0);
-  // All products of the launch have teams of one size.
-  BwdPlan best = plan_products(p, a, sms, 2);
-  const BwdPlan single = plan_products(p, a, sms, 1);
-  if (single.clocks < 0.98 * best.clocks) best = single;
-  for (int i = 0; i < 3; ++i) best.parts[i] = take(best.parts[i]);
-  best.bytes = std::max<size_t>(at, 256);
-  return best;
+  for (int i = 0; i < kProducts; ++i) p.parts[i] = take(p.p[i].part_bytes);
+  p.bytes = std::max<size_t>(at, 256);
+  return p;
 }
 
 }  // namespace
@@ -607,64 +616,57 @@ extern "C" int nb_gated_mlp_bwd(const nb_gated_mlp_bwd_args* args, void* stream)
     g.status = a.status;
   }
 
-  // dx and the weight gradients.
-  GemmParams<4> g{};
+  // dx and the weight gradients, the longer units first.
+  GemmParams<kProducts> g{};
   g.status = a.status;
-  const int hidden_steps = div_up(s.hidden, kGemmDepth), dw_steps = div_up(s.tokens, kGemmDepth);
-  int n = 0, dw_units = 0, dx_units = 0;
-  const auto add_dx = [&]() -> int {
-    if (a.dx.ptr == nullptr) return NB_ATTN_OK;
-    GemmProblem& p = g.p[n++];
-    set_tiles(&p, s.tokens, s.dim, plan.dx, hidden_steps, 2 * hidden_steps);
-    p.b_mn = 1;
-    NB_TRY(map_k_major(&p.a[0], da, s.tokens, s.hidden, kGemmRows));
-    NB_TRY(map_k_major(&p.a[1], db, s.tokens, s.hidden, kGemmRows));
-    NB_TRY(map_mn_major(&p.b[0], a.w_gate, s.hidden, s.dim));
-    NB_TRY(map_mn_major(&p.b[1], a.w_up, s.hidden, s.dim));
-    dx_units = p.row_tiles * p.col_tiles;
-    return host_matrix_map(&p.c, a.dx.ptr, s.tokens, s.dim, a.dx.stride, 32, 64);
-  };
   SplitParams sums{};
-  const auto add_dw = [&](int which, const nb_matrix& left, const nb_matrix& right, const nb_matrix& out) -> int {
-    if (out.ptr == nullptr) return NB_ATTN_OK;
+  int n = 0;
+  const auto add = [&](int which, const nb_matrix& out) -> int {
+    const Product& from = plan.p[which];
+    if (!from.wanted) return NB_ATTN_OK;
+    const bool dx = which == kDx;
     GemmProblem& p = g.p[n++];
-    const int rows = which < 2 ? s.hidden : s.dim, cols = which < 2 ? s.dim : s.hidden;
-    set_tiles(&p, rows, cols, plan.dw[which], dw_steps, dw_steps);
-    p.a_mn = p.b_mn = 1;
-    p.splits = plan.splits[which], p.split_steps = plan.split_steps[which];
-    NB_TRY(map_mn_major(&p.a[0], left, s.tokens, rows));
-    NB_TRY(map_mn_major(&p.b[0], right, s.tokens, cols));
-    dw_units += p.row_tiles * p.col_tiles * p.splits;
-    if (p.splits > 1) {
-      p.partial = reinterpret_cast<float*>(ws + plan.parts[which]);
-      SplitItem& i = sums.item[sums.n_items++];
-      i.partial = reinterpret_cast<const float4*>(p.partial);
-      i.out = static_cast<bf16*>(out.ptr), i.stride = out.stride;
-      i.rows = rows, i.n = cols, i.row_tiles = p.row_tiles * plan.dx.ctas, i.col_tiles = p.col_tiles, i.cols = p.cols;
-      i.splits = p.splits;
-      i.pieces = int64_t(i.row_tiles) * p.col_tiles * (p.cols / 8) * kGemmRows;
-      return NB_ATTN_OK;
+    set_tiles(&p, from.m, from.n, from.tiles, dx ? from.steps / 2 : from.steps, from.steps);
+    p.splits = from.splits, p.split_steps = from.split_steps;
+    p.a_mn = !dx, p.b_mn = 1;
+    if (dx) {
+      NB_TRY(map_k_major(&p.a[0], da, s.tokens, s.hidden, kGemmRows));
+      NB_TRY(map_k_major(&p.a[1], db, s.tokens, s.hidden, kGemmRows));
+      NB_TRY(map_mn_major(&p.b[0], a.w_gate, s.hidden, s.dim));
+      NB_TRY(map_mn_major(&p.b[1], a.w_up, s.hidden, s.dim));
+    } else {
+      NB_TRY(map_mn_major(&p.a[0], which == kDWGate ? da : which == kDWUp ? db : a.dy, s.tokens, from.m));
+      NB_TRY(map_mn_major(&p.b[0], which == kDWDown ? h : a.x, s.tokens, from.n));
     }
-    return host_matrix_map(&p.c, out.ptr, rows, cols, out.stride, 32, 64);
+    if (p.splits == 1) return host_matrix_map(&p.c, out.ptr, from.m, from.n, out.stride, 32, 64);
+    p.partial = reinterpret_cast<float*>(ws + plan.parts[which]);
+    SplitItem& i = sums.item[sums.n_items++];
+    i.partial = reinterpret_cast<const float4*>(p.partial);
+    i.out = static_cast<bf16*>(out.ptr), i.stride = out.stride;
+    i.rows = int(from.m), i.n = from.n, i.row_tiles = p.row_tiles * plan.ctas, i.col_tiles = p.col_tiles, i.cols = p.cols;
+    i.splits = p.splits;
+    i.pieces = int64_t(i.row_tiles) * p.col_tiles * (p.cols / 8) * kGemmRows;
+    return NB_ATTN_OK;
   };
-  // The longer units first.
-  const bool dw_first = std::max({plan.split_steps[0], plan.split_steps[1], plan.split_steps[2]}) >= 2 * hidden_steps;
-  if (!dw_first) NB_TRY(add_dx());
-  NB_TRY(add_dw(0, da, a.x, a.d_w_gate));
-  NB_TRY(add_dw(1, db, a.x, a.d_w_up));
-  NB_TRY(add_dw(2, a.dy, h, a.d_w_down));
-  if (dw_first) NB_TRY(add_dx());
+  const Product &dx = plan.p[kDx], &dw = plan.p[kDWGate];
+  const bool dw_first = dw.unit_clocks() >= dx.unit_clocks();
+  if (!dw_first) NB_TRY(add(kDx, a.dx));
+  NB_TRY(add(kDWGate, a.d_w_gate));
+  NB_TRY(add(kDWUp, a.d_w_up));
+  NB_TRY(add(kDWDown, a.d_w_down));
+  if (dw_first) NB_TRY(add(kDx, a.dx));
   if (dact) NB_TRY(launch_act<kGemmDact>(act, s, act_tiling.ctas, sms, stream));
   if (n > 0) {
-    const int n_long = dw_first ? dw_units : dx_units, n_short = dw_first ? dx_units : dw_units;
-    g.deal.n_long = n_long, g.deal.n_short = n_short;
-    const int teams = std::min(n_long + n_short, sms / plan.dx.ctas), rem = n_long % teams;
-    if (n_short > 0 && rem > 0) {
-      const int dw_len = plan.split_steps[0], dx_len = 2 * hidden_steps;
-      const int ratio = dw_first ? dw_len / dx_len : dx_len / std::max(1, dw_len);
-      g.deal.extra = std::min(ratio, n_short / (teams - rem));
+    int dw_units = 0;
+    for (int i = 0; i < kDx; ++i) dw_units += plan.p[i].wanted ? plan.p[i].units() : 0;
+    const int dx_units = dx.wanted ? dx.units() : 0;
+    g.deal.n_long = dw_first ? dw_units : dx_units, g.deal.n_short = dw_first ? dx_units : dw_units;
+    const int teams = std::min(dw_units + dx_units, sms / plan.ctas), rem = g.deal.n_long % teams;
+    if (g.deal.n_short > 0 && rem > 0) {
+      const double ratio = dw.unit_clocks() / dx.unit_clocks();
+      g.deal.extra = std::min(int(dw_first ? ratio : 1.0 / ratio), g.deal.n_short / (teams - rem));
     }
-    NB_TRY((launch_gemm<kGemmPlain, 0, 0, 4>(g, plan.dx.ctas, sms, stream)));
+    NB_TRY((launch_gemm<kGemmPlain, 0, 0, kProducts>(g, plan.ctas, sms, stream)));
   }
   if (sums.n_items > 0) {
     int64_t pieces = 0;
