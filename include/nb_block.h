@@ -81,7 +81,8 @@ typedef struct nb_gated_mlp_fwd_args {
   nb_gated_mlp_shape shape;
   nb_matrix x, w_gate, w_up, w_down, y;
   const void *b_gate, *b_up, *b_down;
-  nb_matrix h;      /* [tokens][hidden]: the product in front of Wd; the backward wants it unless the checkpoint has 8 bits */
+  nb_matrix h;      /* [tokens][hidden]: the product in front of Wd; the backward wants it unless the checkpoint has 8 bits.
+                     * A stride that is a multiple of 64 is faster */
   void* checkpoint; /* nb_gated_mlp_checkpoint_bytes(&shape) bytes, 256-byte aligned */
   int32_t* status;
 } nb_gated_mlp_fwd_args;

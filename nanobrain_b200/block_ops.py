@@ -71,7 +71,7 @@ def _define_ops() -> torch.library.Library:
     def _(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation, checkpoint):
         hidden = w_gate.shape[0]
         tokens = x.numel() // x.shape[-1]
-        h = x.new_empty((tokens, hidden) if checkpoint == 1 else (0,))
+        h = x.new_empty((tokens, -(-hidden // 64) * 64))[:, :hidden] if checkpoint == 1 else x.new_empty((0,))
         codes = x.new_empty((_checkpoint_bytes(tokens, hidden, checkpoint),), dtype=torch.uint8)
         return x.new_empty(x.shape), h, codes
 

@@ -297,14 +297,19 @@ Three mlp_fwd_cuda(const Tensor& x_, const Tensor& w_gate_, const Tensor& w_up_,
                w_down = rows_of(w_down_, hidden);
   nb_gated_mlp_fwd_args a{};
   a.shape = {tokens, int32_t(dim), int32_t(hidden), int32_t(activation), int32_t(checkpoint)};
-  Tensor y = new_tensor(x_.sizes(), at::kBFloat16, x), h = new_tensor({tokens, hidden}, at::kBFloat16, x);
+  // Rows of h begin on lines of 128 bytes: with 1368 features side by side the product with w_down takes 160 instead of 132
+  // us (131072 tokens, dim 512).
+  const int64_t stride = (hidden + 63) / 64 * 64;
+  Tensor y = new_tensor(x_.sizes(), at::kBFloat16, x), h = new_tensor({tokens, stride}, at::kBFloat16, x);
   Tensor codes = new_tensor({int64_t(nb_gated_mlp_checkpoint_bytes(&a.shape))}, at::kByte, x);
   const auto result = [&]() -> Three {  // the backward wants h from 16 bits; in 8 bits it makes h again
-    return {y, checkpoint == NB_CHECKPOINT_16BIT ? h : new_tensor({0}, at::kBFloat16, x), codes};
+    if (checkpoint != NB_CHECKPOINT_16BIT) h = new_tensor({0}, at::kBFloat16, x);
+    else if (stride != hidden) h = h.narrow(1, 0, hidden);
+    return {y, h, codes};
   };
   if (tokens == 0) return result();
   a.x = matrix(x), a.w_gate = matrix(w_gate), a.w_up = matrix(w_up), a.w_down = matrix(w_down);
-  a.y = {y.data_ptr(), dim}, a.h = {h.data_ptr(), hidden};
+  a.y = {y.data_ptr(), dim}, a.h = {h.data_ptr(), stride};
   a.b_gate = address(b_gate), a.b_up = address(b_up), a.b_down = address(b_down);
   if (checkpoint != NB_CHECKPOINT_NONE) a.checkpoint = codes.data_ptr();
   volatile int32_t* word = nbt::status_ptr(x.get_device());
