@@ -4,7 +4,7 @@
 //   kGemmDact   dh = dy Wd; with a and b from the checkpoint da = dh b act'(a) and db = dh act(a) leave (and h again)
 //   kGemmPlain  up to four products of one launch, e.g. dx = da Wg + db Wu, dWg = da^T x, dWu = db^T x, dWd = dy^T h
 //
-// One persistent CTA per SM: warp 0 drives TMA, one thread of warp 1 issues tcgen05.mma, warps 4-11 are two epilogue
+// One persistent CTA per SM: warps 0 and 2 drive TMA, one thread of warp 1 issues tcgen05.mma, warps 4-11 are two epilogue
 // warpgroups. A unit is an output tile of 128 rows x up to 256 columns over a range of 64-deep steps. A and B tiles
 // are 64 elements (128 bytes, swizzled) x rows whichever way the matrix lies in memory: where the inner index runs
 // along memory the tile is a K-major operand, otherwise an MN-major one, so no product needs a transposed copy.
@@ -316,10 +316,22 @@ __device__ __forceinline__ void add_bias32(float (&v)[32], const __nv_bfloat16* 
   }
 }
 
+// The wait for a load from tensor memory, as something that its registers depend on: nothing computed from them may be
+// moved in front of it.
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                 "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                 "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28])
+               :
+               : "memory");
+  asm volatile("" : "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) : : "memory");
+}
 __device__ __forceinline__ void tmem_ld32f(uint32_t taddr, float (&v)[32]) {
   uint32_t r[32];
   tmem_ld32(taddr, r);
-  tmem_wait_ld();
+  tmem_wait_ld32(r);
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
@@ -383,65 +395,66 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
 
   const GemmTurns<kCtas> turns(g.deal);
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp == 0 || warp == 2) {
+    // One thread loads A's tiles, another one B's, both elected: issuing a step's four loads of MN-major blocks took a single
+    // thread, chosen by its lane, nearly the 512 clocks of the step's MMAs (dx and the weight gradients of 26253 x 768 x 2048:
+    // 300 us; two threads chosen by their lanes 316, as they look at what their waits return; two elected ones 267).
+    if (elect_one()) {
+      const bool for_a = warp == 0;
       const auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
         if constexpr (kPair) tma_load_2d_pair(dst, map, bar, c0, c1);
         else tma_load_2d(dst, map, bar, c0, c1);
       };
       int stage = 0;
       uint32_t phase = 0;
-      for (int i = 0;; ++i) {
+      // It ends where one of its waits gave up: more arrivals than a phase expects, while bytes are due, are not defined.
+      bool live = true;
+      for (int i = 0; live; ++i) {
         const int id = turns.unit(i);
         if (id < 0) break;
         const GemmUnit u = gemm_unit(g, id);
         const GemmProblem& p = g.p[u.problem];
         const int cols = p.cols, mine = cols / kCtas;  // columns of the tile, and those that this CTA loads
-        const int row0 = (u.row * kCtas + rank) * kGemmRows, col0 = u.col * cols + rank * mine;
-        // (B's tile in blocks of 64 columns where its columns run along memory: a pair's 96 take two blocks)
-        const int loaded = p.b_mn ? (mine + 63) / 64 * 64 : mine;
-        const uint32_t bytes = kCtas * (kGemmBytesA + uint32_t(loaded) * (kGemmDepth * 2));
+        const int row0 = (u.row * kCtas + rank) * kGemmRows, steps0 = p.steps0;
+        // Blocks of 64 columns of an MN-major tile (a pair's 96 take two), 0: a K-major one.
+        const int a_blocks = p.a_mn ? 2 : 0, b_blocks = p.b_mn ? (mine + 63) / 64 : 0;
+        const uint32_t bytes = kCtas * (kGemmBytesA + uint32_t(b_blocks ? b_blocks * 64 : mine) * (kGemmDepth * 2));
+        // The gate's tile has columns of a, then as many of b: in a pair rank 0 holds those of a and rank 1 those of b.
+        const int half = cols / 2, col0 = kKind == kGemmGate ? u.col * half : u.col * cols + rank * mine;
+        const CUtensorMap* map = for_a ? &p.a[0] : &p.b[kKind == kGemmGate && kPair ? rank : 0];
+        const int blocks = for_a ? a_blocks : b_blocks, first = for_a ? row0 : col0;
         for (int s = u.begin; s < u.end; ++s) {
-          mbar_wait(empty + 8 * stage, phase ^ 1, abort_flag);
-          const uint32_t at_a = base + stage * L::kStageBytes, at_b = at_a + kGemmBytesA;
+          live = mbar_wait(empty + 8 * stage, phase ^ 1, abort_flag);
+          if (!live) break;
+          const uint32_t at = base + stage * L::kStageBytes + (for_a ? 0 : kGemmBytesA);
           uint32_t bar = full + 8 * stage;
-          if (rank == 0) mbar_arrive_expect_tx(bar, bytes);  // (of both CTAs: all loads count on rank 0's barrier)
+          if (for_a && rank == 0) mbar_arrive_expect_tx(bar, bytes);  // (all loads of both CTAs count on rank 0's barrier)
           if constexpr (kPair) bar = map_to_rank(bar, 0);
-          const int second = s >= p.steps0;
-          const int k = (second ? s - p.steps0 : s) * kGemmDepth;
-          if (p.a_mn) {
-            for (int b = 0; b < 2; ++b) load(at_a + b * 8192, &p.a[second], bar, row0 + b * 64, k);
+          const int second = kKind == kGemmPlain && s >= steps0;
+          const int k = (second ? s - steps0 : s) * kGemmDepth;
+          if (blocks) {
+            for (int b = 0; b < blocks; ++b) load(at + b * 8192, map + second, bar, first + b * 64, k);
           } else {
-            load(at_a, &p.a[second], bar, k, row0);
-          }
-          if constexpr (kKind == kGemmGate) {
-            // Columns of a, then as many of b: in a pair rank 0 holds those of a and rank 1 those of b.
-            const int half = cols / 2;
-            if constexpr (kPair) {
-              load(at_b, &p.b[rank], bar, k, u.col * half);
-            } else {
-              load(at_b, &p.b[0], bar, k, u.col * half);
-              load(at_b + half * 128, &p.b[1], bar, k, u.col * half);
-            }
-          } else if (p.b_mn) {
-            for (int b = 0; b < loaded / 64; ++b) load(at_b + b * 8192, &p.b[second], bar, col0 + b * 64, k);
-          } else {
-            load(at_b, &p.b[second], bar, k, col0);
+            load(at, map + second, bar, k, first);
+            if constexpr (kKind == kGemmGate && !kPair)
+              if (!for_a) load(at + half * 128, map + 1, bar, k, first);
           }
           if (++stage == kStages) stage = 0, phase ^= 1;
         }
       }
       if constexpr (kPair) {  // rank 0's arrivals on this CTA's barriers are in before it may end
-        for (int s = 0; s < kStages; ++s) {
-          mbar_wait(empty + 8 * stage, phase ^ 1, abort_flag);
+        for (int s = 0; s < kStages && live; ++s) {
+          live = mbar_wait(empty + 8 * stage, phase ^ 1, abort_flag);
           if (++stage == kStages) stage = 0, phase ^= 1;
         }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0 && elect_one()) {
       int stage = 0;
       uint32_t phase = 0;
+      // (No look at what the waits return: a test between wait and MMAs made the products 30 % slower, and behind a wait that
+      // gave up these MMAs and arrivals, each a whole phase of its barrier, do no harm.)
       for (int i = 0;; ++i) {
         const int id = turns.unit(i);
         if (id < 0) break;
@@ -513,13 +526,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     if constexpr (kKind == kGemmDact)
       for (int i = 0; i < L::kSlots; ++i) request(i);
 
-    for (int i = 0;; ++i) {
+    [[maybe_unused]] bool live = true;
+    for (int i = 0; live; ++i) {
       const int id = turns.unit(i);
       if (id < 0) break;
       const GemmUnit u = gemm_unit(g, id);
       const GemmProblem& p = g.p[u.problem];
       const uint32_t acc = tmem + lanes + (i & 1) * kGemmMaxCols;
-      mbar_wait(acc_full + 8 * (i & 1), (i >> 1) & 1, abort_flag);
+      if (!__all_sync(0xffffffffu, mbar_wait(acc_full + 8 * (i & 1), (i >> 1) & 1, abort_flag))) break;
       tc_fence_after();
       const int row0 = rows_of(u), row = row0 + quarter * 32;  // of the tile, of the warp
       if (kPair && row0 >= p.m) {
@@ -576,7 +590,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
           const int f = u.col * p.cols + blk;
           if (f >= g.hidden) break;
           const uint32_t slot = piece % L::kSlots, codes = own + L::kBoxes + slot * Block::kBytes;
-          mbar_wait(my_codes + 8 * slot, (piece / L::kSlots) & 1, abort_flag);
+          live = __all_sync(0xffffffffu, mbar_wait(my_codes + 8 * slot, (piece / L::kSlots) & 1, abort_flag));
+          if (!live) break;
           uint32_t scales;
           asm volatile("ld.shared.b32 %0, [%1];" : "=r"(scales) : "r"(codes + Block::kScales + lane * 4) : "memory");
           const float2 sa = both(__uint_as_float(scales << 16)), sb = both(__uint_as_float(scales & 0xFFFF0000u));
@@ -591,7 +606,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
           }
           __syncwarp();
           request(slot);  // the block has been read
-          tmem_wait_ld();
+          tmem_wait_ld32(r);
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             float d[16], e[16];
@@ -672,6 +687,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
           }
         }
       }
+      if (!live) break;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {

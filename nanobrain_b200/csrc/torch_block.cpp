@@ -75,7 +75,10 @@ void check_qk(const Tensor& q, const Tensor& k) {
   QK_REQUIRE(q.device() == k.device(), "q and k must be on the same device");
   QK_REQUIRE(q.dim() == k.dim(), "q and k must both be packed or both dense");
   QK_REQUIRE(q.dim() == 3 || q.size(0) == k.size(0), "q and k must agree on the batch");
-  QK_REQUIRE(q.size(1) > 0 && k.size(1) > 0, "there must be at least one head");
+  for (const Tensor& t : {q, k}) {
+    QK_REQUIRE(t.size(1) > 0 && t.size(1) <= 65535, "there must be 1 to 65535 heads, got ", t.size(1));
+    QK_REQUIRE(t.numel() / (t.size(1) * kHeadDim) <= INT32_MAX, "there must be fewer than 2^31 tokens");
+  }
 }
 
 void set_side(QkCall& c, nb_qk_side& s, const Tensor& x, const MaybeTensor& weight, const char* weight_name,
@@ -260,6 +263,7 @@ void check_mlp(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const 
               ", ", hidden, "], got ", w_down.sizes());
   MLP_REQUIRE(dim > 0 && hidden > 0 && dim % 8 == 0 && hidden % 8 == 0, "dim and hidden must be multiples of 8, got ", dim,
               " and ", hidden);
+  MLP_REQUIRE(dim <= 1 << 20 && hidden <= 1 << 20, "dim and hidden must be 2^20 at most, got ", dim, " and ", hidden);
   MLP_REQUIRE(activation == NB_ACT_SILU || activation == NB_ACT_GELU, "no such activation");
 }
 
