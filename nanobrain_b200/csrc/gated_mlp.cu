@@ -18,23 +18,26 @@ using namespace nb;
 using bf16 = __nv_bfloat16;
 
 // ---- few tokens, forward only ----------------------------------------------------------------
-// Bound by reading the weights once: a warp takes a feature (a row of Wg and of Wu, or of Wd), its lanes 16 bytes at a
-// time, and applies it to all tokens. On tensor cores the 4096 weight rows of ViT-B's block would occupy 32 of 148 SMs.
-constexpr int kFewTokens = 8, kFewWarps = 4;
+// Bound by reading the weights once, from as many SMs and with as many loads under way as there can be: a block takes 16
+// features (rows of Wg and Wu, or of Wd), its warps deal their 32-deep chunks out, and the block adds the warps' sums up.
+// The products are mma.sync's of 16 features x 8 tokens: with one token per multiply-add the time grew with the tokens
+// (768 x 2048, weights from memory, us: 1 token 7.1, 8 tokens 29; now 6.7, 7.2, 16 tokens 9.3), and the tiles of the large
+// kernels occupy 16 to 48 SMs (17 for up to 128 tokens, and so faster from 17 tokens on: 32 tokens take 20 here). A
+// lane's 16 bytes are eight neighbouring k of its row; the order of k inside a chunk does not matter as long as weights and
+// tokens have the same.
+constexpr int kFewTokens = 16, kFewRows = 16;
+constexpr int kFewGateWarps = 8, kFewDownWarps = 16;
 
-__device__ __forceinline__ float dot8(const uint4& w, const uint4& x, float acc) {
-  const uint32_t a[4] = {w.x, w.y, w.z, w.w}, b[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    acc = fmaf(__uint_as_float(a[i] << 16), __uint_as_float(b[i] << 16), acc);
-    acc = fmaf(__uint_as_float(a[i] & 0xFFFF0000u), __uint_as_float(b[i] & 0xFFFF0000u), acc);
-  }
-  return acc;
+__device__ __forceinline__ void mma_16x8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-  return v;
+// 32 deep: rows g and g + 8 of the features, row g of the tokens.
+__device__ __forceinline__ void mma_chunk(float (&c)[4], const uint4& lo, const uint4& hi, const uint4& x) {
+  mma_16x8(c, lo.x, hi.x, lo.y, hi.y, x.x, x.y);
+  mma_16x8(c, lo.z, hi.z, lo.w, hi.w, x.z, x.w);
 }
 
 struct FewParams {
@@ -44,79 +47,99 @@ struct FewParams {
   int32_t tokens, in, out_n;
 };
 
-template <int kAct, int kTokens>
-__global__ void __launch_bounds__(kFewWarps * 32) few_gate_kernel(const __grid_constant__ FewParams p) {
-  pdl_wait();
-  pdl_launch_dependents();
-  const int lane = threadIdx.x & 31, f = blockIdx.x * kFewWarps + (threadIdx.x >> 5);
-  if (f >= p.out_n) return;
-  const bf16 *wg = p.w0 + f * p.w0s, *wu = p.w1 + f * p.w1s;
-  float a[kTokens], b[kTokens];
-#pragma unroll
-  for (int t = 0; t < kTokens; ++t) a[t] = b[t] = 0.f;
-#pragma unroll 4
-  for (int c = lane * 8; c < p.in; c += 256) {
-    const uint4 g = *reinterpret_cast<const uint4*>(wg + c), u = *reinterpret_cast<const uint4*>(wu + c);
-#pragma unroll
-    for (int t = 0; t < kTokens; ++t) {
-      if (t >= p.tokens) break;
-      const uint4 x = *reinterpret_cast<const uint4*>(p.x + t * p.xs + c);
-      a[t] = dot8(g, x, a[t]), b[t] = dot8(u, x, b[t]);
-    }
-  }
-#pragma unroll
-  for (int t = 0; t < kTokens; ++t) a[t] = warp_sum(a[t]), b[t] = warp_sum(b[t]);
-  if (lane != 0) return;
-  const float bg = p.bias0 != nullptr ? __bfloat162float(p.bias0[f]) : 0.f;
-  const float bu = p.bias1 != nullptr ? __bfloat162float(p.bias1[f]) : 0.f;
-#pragma unroll
-  for (int t = 0; t < kTokens; ++t)
-    if (t < p.tokens) p.out[t * p.outs + f] = __float2bfloat16(gate_of<kAct>(a[t] + bg) * (b[t] + bu));
+// 16 bytes of row `row`, zeros behind the last row or column.
+__device__ __forceinline__ uint4 few_load(const bf16* m, int64_t stride, int row, int rows, int k, int n) {
+  return row < rows && k < n ? *reinterpret_cast<const uint4*>(m + row * stride + k) : make_uint4(0, 0, 0, 0);
 }
 
-constexpr int kFewAhead = 8;  // pieces of a lane's weights requested before the kernel in front is done
-template <int kTokens>
-__global__ void __launch_bounds__(kFewWarps * 32) few_down_kernel(const __grid_constant__ FewParams p) {
-  const int lane = threadIdx.x & 31, d = blockIdx.x * kFewWarps + (threadIdx.x >> 5);
-  const bf16* w = p.w0 + int64_t(min(d, p.out_n - 1)) * p.w0s;
+// Adds up the warps' sums of output i = (token, feature) of the block.
+template <int kWarps, int kTiles>
+__device__ __forceinline__ float few_total(const float (&part)[kWarps][kFewRows][8 * kTiles], int token, int feature) {
+  float v = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) v += part[w][feature][token];
+  return v;
+}
+template <int kWarps, int kTiles>
+__device__ __forceinline__ void few_put(float (&part)[kWarps][kFewRows][8 * kTiles], const float (&acc)[kTiles][4], int warp,
+                                        int lane) {
+  const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i) {
+    part[warp][g][8 * i + 2 * t] = acc[i][0], part[warp][g][8 * i + 2 * t + 1] = acc[i][1];
+    part[warp][g + 8][8 * i + 2 * t] = acc[i][2], part[warp][g + 8][8 * i + 2 * t + 1] = acc[i][3];
+  }
+}
+
+template <int kAct, int kTiles>  // tiles of eight tokens
+__global__ void __launch_bounds__(kFewGateWarps * 32) few_gate_kernel(const __grid_constant__ FewParams p) {
+  __shared__ float part_a[kFewGateWarps][kFewRows][8 * kTiles], part_b[kFewGateWarps][kFewRows][8 * kTiles];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, f0 = blockIdx.x * kFewRows;
+  float a[kTiles][4] = {}, b[kTiles][4] = {};
+#pragma unroll 3
+  for (int k = warp * 32 + (lane & 3) * 8; k < (p.in + 31) / 32 * 32; k += kFewGateWarps * 32) {
+    const uint4 g0 = few_load(p.w0, p.w0s, f0 + g, p.out_n, k, p.in), g1 = few_load(p.w0, p.w0s, f0 + g + 8, p.out_n, k, p.in);
+    const uint4 u0 = few_load(p.w1, p.w1s, f0 + g, p.out_n, k, p.in), u1 = few_load(p.w1, p.w1s, f0 + g + 8, p.out_n, k, p.in);
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      const uint4 x = few_load(p.x, p.xs, 8 * i + g, p.tokens, k, p.in);
+      mma_chunk(a[i], g0, g1, x);
+      mma_chunk(b[i], u0, u1, x);
+    }
+  }
+  few_put(part_a, a, warp, lane);
+  few_put(part_b, b, warp, lane);
+  __syncthreads();
+  for (int i = threadIdx.x; i < kFewRows * 8 * kTiles; i += kFewGateWarps * 32) {
+    const int token = i / kFewRows, feature = i % kFewRows, f = f0 + feature;
+    if (token >= p.tokens || f >= p.out_n) continue;
+    const float bg = p.bias0 != nullptr ? __bfloat162float(p.bias0[f]) : 0.f;
+    const float bu = p.bias1 != nullptr ? __bfloat162float(p.bias1[f]) : 0.f;
+    const float va = few_total<kFewGateWarps, kTiles>(part_a, token, feature) + bg;
+    const float vb = few_total<kFewGateWarps, kTiles>(part_b, token, feature) + bu;
+    p.out[token * p.outs + f] = __float2bfloat16(gate_of<kAct>(va) * vb);
+  }
+}
+
+constexpr int kFewAhead = 4;  // chunks of a warp's weights requested before the kernel in front is done
+template <int kTiles>
+__global__ void __launch_bounds__(kFewDownWarps * 32) few_down_kernel(const __grid_constant__ FewParams p) {
+  __shared__ float part[kFewDownWarps][kFewRows][8 * kTiles];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, d0 = blockIdx.x * kFewRows;
+  const int k0 = warp * 32 + (lane & 3) * 8;
+  constexpr int kStep = kFewDownWarps * 32;
   // The gate kernel, which comes right in front, does not write weights.
-  uint4 ahead[kFewAhead];
+  uint4 lo[kFewAhead], hi[kFewAhead];
 #pragma unroll
   for (int i = 0; i < kFewAhead; ++i) {
-    const int c = lane * 8 + i * 256;
-    ahead[i] = c < p.in ? *reinterpret_cast<const uint4*>(w + c) : make_uint4(0, 0, 0, 0);
+    lo[i] = few_load(p.w0, p.w0s, d0 + g, p.out_n, k0 + i * kStep, p.in);
+    hi[i] = few_load(p.w0, p.w0s, d0 + g + 8, p.out_n, k0 + i * kStep, p.in);
   }
   pdl_wait();
   pdl_launch_dependents();
-  float y[kTokens];
-#pragma unroll
-  for (int t = 0; t < kTokens; ++t) y[t] = 0.f;
+  float y[kTiles][4] = {};
 #pragma unroll
   for (int i = 0; i < kFewAhead; ++i) {
-    const int c = lane * 8 + i * 256;
-    if (c >= p.in) break;
+    if (warp * 32 + i * kStep >= p.in) break;
 #pragma unroll
-    for (int t = 0; t < kTokens; ++t) {
-      if (t >= p.tokens) break;
-      y[t] = dot8(ahead[i], *reinterpret_cast<const uint4*>(p.x + t * p.xs + c), y[t]);
-    }
+    for (int t = 0; t < kTiles; ++t) mma_chunk(y[t], lo[i], hi[i], few_load(p.x, p.xs, 8 * t + g, p.tokens, k0 + i * kStep, p.in));
   }
-#pragma unroll 4
-  for (int c = lane * 8 + kFewAhead * 256; c < p.in; c += 256) {
-    const uint4 g = *reinterpret_cast<const uint4*>(w + c);
+#pragma unroll 2
+  for (int k = k0 + kFewAhead * kStep; k < (p.in + 31) / 32 * 32; k += kStep) {
+    const uint4 w0 = few_load(p.w0, p.w0s, d0 + g, p.out_n, k, p.in), w1 = few_load(p.w0, p.w0s, d0 + g + 8, p.out_n, k, p.in);
 #pragma unroll
-    for (int t = 0; t < kTokens; ++t) {
-      if (t >= p.tokens) break;
-      y[t] = dot8(g, *reinterpret_cast<const uint4*>(p.x + t * p.xs + c), y[t]);
-    }
+    for (int t = 0; t < kTiles; ++t) mma_chunk(y[t], w0, w1, few_load(p.x, p.xs, 8 * t + g, p.tokens, k, p.in));
   }
-#pragma unroll
-  for (int t = 0; t < kTokens; ++t) y[t] = warp_sum(y[t]);
-  if (lane != 0 || d >= p.out_n) return;
-  const float bias = p.bias0 != nullptr ? __bfloat162float(p.bias0[d]) : 0.f;
-#pragma unroll
-  for (int t = 0; t < kTokens; ++t)
-    if (t < p.tokens) p.out[t * p.outs + d] = __float2bfloat16(y[t] + bias);
+  few_put(part, y, warp, lane);
+  __syncthreads();
+  for (int i = threadIdx.x; i < kFewRows * 8 * kTiles; i += kFewDownWarps * 32) {
+    const int token = i / kFewRows, feature = i % kFewRows, d = d0 + feature;
+    if (token >= p.tokens || d >= p.out_n) continue;
+    const float bias = p.bias0 != nullptr ? __bfloat162float(p.bias0[d]) : 0.f;
+    p.out[token * p.outs + d] = __float2bfloat16(few_total<kFewDownWarps, kTiles>(part, token, feature) + bias);
+  }
 }
 
 // ---- what is left in parts ---------------------------------------------------------------------
@@ -357,7 +380,7 @@ int map_mn_major(CUtensorMap* m, const nb_matrix& t, int64_t rows, int64_t cols)
     if (const int rc_ = (expr)) return rc_; \
   } while (0)
 
-template <int kAct, int kTokens>
+template <int kAct, int kTiles>
 int launch_few(const nb_gated_mlp_fwd_args& a, void* stream) {
   const nb_gated_mlp_shape& s = a.shape;
   FewParams p{};
@@ -367,20 +390,18 @@ int launch_few(const nb_gated_mlp_fwd_args& a, void* stream) {
   p.bias0 = static_cast<const bf16*>(a.b_gate), p.bias1 = static_cast<const bf16*>(a.b_up);
   p.out = static_cast<bf16*>(a.h.ptr), p.outs = a.h.stride;
   p.tokens = int(s.tokens), p.in = s.dim, p.out_n = s.hidden;
-  NB_TRY(launch(few_gate_kernel<kAct, kTokens>, dim3(div_up(s.hidden, kFewWarps)), kFewWarps * 32, 0, stream, p));
+  NB_TRY(launch(few_gate_kernel<kAct, kTiles>, dim3(div_up(s.hidden, kFewRows)), kFewGateWarps * 32, 0, stream, p));
   FewParams d{};
   d.x = p.out, d.xs = p.outs;
   d.w0 = static_cast<const bf16*>(a.w_down.ptr), d.w0s = a.w_down.stride;
   d.bias0 = static_cast<const bf16*>(a.b_down);
   d.out = static_cast<bf16*>(a.y.ptr), d.outs = a.y.stride;
   d.tokens = int(s.tokens), d.in = s.hidden, d.out_n = s.dim;
-  return launch(few_down_kernel<kTokens>, dim3(div_up(s.dim, kFewWarps)), kFewWarps * 32, 0, stream, d);
+  return launch(few_down_kernel<kTiles>, dim3(div_up(s.dim, kFewRows)), kFewDownWarps * 32, 0, stream, d);
 }
 template <int kAct>
 int launch_few(const nb_gated_mlp_fwd_args& a, void* stream) {
-  if (a.shape.tokens == 1) return launch_few<kAct, 1>(a, stream);
-  if (a.shape.tokens == 2) return launch_few<kAct, 2>(a, stream);
-  return a.shape.tokens <= 4 ? launch_few<kAct, 4>(a, stream) : launch_few<kAct, kFewTokens>(a, stream);
+  return a.shape.tokens <= 8 ? launch_few<kAct, 1>(a, stream) : launch_few<kAct, 2>(a, stream);
 }
 
 template <int kKind, int kAct>

@@ -77,8 +77,9 @@ def test_training_against_64_bits(tokens, dim, hidden, activation, bias, checkpo
     compare(args, activation, checkpoint, run(args, dy, activation, checkpoint), dy)
 
 
-@pytest.mark.parametrize("tokens", [1, 2, 3, 4, 5, 8, 9, 100, 700])
-@pytest.mark.parametrize("dim,hidden,activation,bias", [(768, 2048, "silu", False), (264, 72, "gelu", True), (8, 16, "silu", True)])
+@pytest.mark.parametrize("tokens", [1, 2, 3, 4, 5, 8, 9, 15, 16, 17, 100, 700])
+@pytest.mark.parametrize("dim,hidden,activation,bias", [(768, 2048, "silu", False), (264, 72, "gelu", True), (8, 16, "silu", True),
+                                                        (2320, 1000, "silu", True)])
 def test_inference_against_64_bits(tokens, dim, hidden, activation, bias):
     args = problem(tokens, dim, hidden, bias)
     with torch.inference_mode():
