@@ -444,11 +444,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
           if (++stage == kStages) stage = 0, phase ^= 1;
         }
       }
-      if constexpr (kPair) {  // rank 0's arrivals on this CTA's barriers are in before it may end
-        for (int s = 0; s < kStages && live; ++s) {
-          live = mbar_wait(empty + 8 * stage, phase ^ 1, abort_flag);
-          if (++stage == kStages) stage = 0, phase ^= 1;
-        }
+      // The MMAs' arrivals on this CTA's barriers (rank 0's in a pair) are in before it may end.
+      for (int s = 0; s < kStages && live; ++s) {
+        live = mbar_wait(empty + 8 * stage, phase ^ 1, abort_flag);
+        if (++stage == kStages) stage = 0, phase ^= 1;
       }
     }
   } else if (warp == 1) {
@@ -710,6 +709,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     if constexpr (kPair) tmem_dealloc_pair(tmem, 512);
     else tmem_dealloc(tmem, 512);
   }
+  // Neither SM of a pair takes a block of the next kernel, which may want tensor memory for itself, before both CTAs have
+  // given theirs back.
+  __syncwarp();
+  if constexpr (kPair) cluster_sync();
 }
 
 }  // namespace nb
