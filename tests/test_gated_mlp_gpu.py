@@ -90,6 +90,18 @@ def test_inference_against_64_bits(tokens, dim, hidden, activation, bias):
         assert torch.equal(nb.gated_mlp(*args, activation=activation, checkpoint="8bit"), y)
 
 
+@pytest.mark.parametrize("tokens", [17, 129, 300, 500, 1200, 2000, 3000])
+@pytest.mark.parametrize("dim,hidden", [(1024, 2736), (512, 1368), (128, 344)])
+def test_inference_in_every_tiling(tokens, dim, hidden):
+    # single CTAs and pairs, tiles of 64 to 256 columns, in launches that follow on one another
+    args = problem(tokens, dim, hidden, False)
+    with torch.inference_mode():
+        calls = [nb.gated_mlp(*args) for _ in range(4)]
+    ops.check_status()
+    close(calls[0], O.mlp(*args)[0], 2)
+    assert all(torch.equal(calls[0], y) for y in calls)
+
+
 @pytest.mark.parametrize("tokens,dim,hidden", [(20000, 64, 72), (6000, 256, 680), (2500, 768, 2048)])
 def test_many_tokens_twice_the_same_bits(tokens, dim, hidden):
     # weight gradients over many tokens (products cut into parts), more tiles than CTAs
