@@ -11,7 +11,8 @@ interleaved=False)``
     ``(act(x @ w_gate.T + b_gate) * (x @ w_up.T + b_up)) @ w_down.T + b_down``, the gated form of the
     reference's two-layer MLP (``src/nanobrain/modules.py:68-85``).
 
-Both take bfloat16 CUDA tensors and have their backward. As in :mod:`nanobrain_b200.ops` the CUDA and autograd
+Both take bfloat16 CUDA tensors and have their backward (once; a tensor that carries a forward-mode tangent is
+refused). As in :mod:`nanobrain_b200.ops` the CUDA and autograd
 kernels are native code (``csrc/torch_block.cpp``), schemas and fake kernels are here, and what is outside the
 supported subset raises: there is no fallback.
 """

@@ -220,6 +220,7 @@ struct QkFunction : public torch::autograd::Function<QkFunction> {
 Two qk_fwd_autograd(const Tensor& q, const Tensor& k, const MaybeTensor& q_weight, const MaybeTensor& k_weight,
                     const MaybeTensor& positions, const MaybeTensor& k_positions, const MaybeTensor& freqs, double eps,
                     bool interleaved) {
+  nbt::refuse_tangents("qk_norm_rope", q, k, q_weight, k_weight, positions, k_positions, freqs);
   if (at::GradMode::is_enabled()) {
     QK_REQUIRE(!differentiable(positions) && !differentiable(k_positions) && !differentiable(freqs),
                "there is no gradient for positions and freqs");
@@ -428,6 +429,7 @@ bool wants_grad(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const
 Three mlp_fwd_autograd(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const Tensor& w_down,
                        const MaybeTensor& b_gate, const MaybeTensor& b_up, const MaybeTensor& b_down, int64_t activation,
                        int64_t checkpoint) {
+  nbt::refuse_tangents("gated_mlp", x, w_gate, w_up, w_down, b_gate, b_up, b_down);
   if (!wants_grad(x, w_gate, w_up, w_down, b_gate, b_up, b_down)) {
     at::AutoDispatchBelowADInplaceOrView guard;
     return mlp_fwd_op().call(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation, checkpoint);

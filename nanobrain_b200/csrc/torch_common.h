@@ -5,6 +5,8 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <torch/extension.h>
 
+#include <optional>
+
 #include "../../include/nb_attn.h"
 
 namespace nbt {
@@ -19,6 +21,16 @@ void check_rc(int rc, const char* what);
 
 void bind_encoder(pybind11::module_& m);
 void bind_block(pybind11::module_& m);
+
+// Forward-mode derivatives: does the tensor carry a tangent? (There is one level, 0.) No operator here has them, and a
+// call below autograd would drop the tangent, which reads as a derivative of zero.
+inline bool has_tangent(const at::Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+inline bool has_tangent(const std::optional<at::Tensor>& t) { return t.has_value() && has_tangent(*t); }
+template <typename... T>
+void refuse_tangents(const char* op, const T&... tensors) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(tensors) || ...), "nanobrain_b200.", op,
+                              ": there are no forward-mode derivatives, but an argument carries a tangent");
+}
 
 // ------------------------------------------------------------------------------------------
 // Layouts
