@@ -12,9 +12,9 @@ interleaved=False)``
     reference's two-layer MLP (``src/nanobrain/modules.py:68-85``).
 
 Both take bfloat16 CUDA tensors and have their backward (once; a tensor that carries a forward-mode tangent is
-refused). As in :mod:`nanobrain_b200.ops` the CUDA and autograd
-kernels are native code (``csrc/torch_block.cpp``), schemas and fake kernels are here, and what is outside the
-supported subset raises: there is no fallback.
+refused). As in :mod:`nanobrain_b200.ops` the CUDA and autograd kernels are native code
+(``csrc/torch_block.cpp``), schemas and fake kernels are here, and what is outside the supported subset raises:
+there is no fallback.
 """
 
 from __future__ import annotations

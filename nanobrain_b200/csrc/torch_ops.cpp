@@ -346,6 +346,7 @@ struct SdpaVarlenFunction : public torch::autograd::Function<SdpaVarlenFunction>
 };
 
 Two sdpa_fwd_autograd(const Tensor& q, const Tensor& k, const Tensor& v, double scale) {
+  nbt::refuse_tangents("sdpa", q, k, v);
   if (!wants_grad(q, k, v)) {
     at::AutoDispatchBelowADInplaceOrView guard;
     return fwd_op().call(q, k, v, scale);
@@ -356,6 +357,7 @@ Two sdpa_fwd_autograd(const Tensor& q, const Tensor& k, const Tensor& v, double 
 
 Two sdpa_varlen_fwd_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_q, const Tensor& cu_k,
                              c10::SymInt max_q, c10::SymInt max_k, double scale) {
+  nbt::refuse_tangents("sdpa_varlen", q, k, v);
   if (!wants_grad(q, k, v)) {
     at::AutoDispatchBelowADInplaceOrView guard;
     return varlen_fwd_op().call(q, k, v, cu_q, cu_k, max_q, max_k, scale);

@@ -18,7 +18,8 @@ Anything outside that subset raises; there is no fallback and no backend dispatc
 (forward and backward of both) have their CUDA and autograd kernels in native code
 (``csrc/torch_ops.cpp``) and their schemas and fake (meta) kernels here, so they trace under
 ``torch.compile`` and ``loss.backward()`` reaches the CUDA backward
-(``src/nanobrain/misc.py:368-371``).
+(``src/nanobrain/misc.py:368-371``). There is no forward-mode derivative: a tensor that carries a tangent is
+refused.
 """
 
 from __future__ import annotations

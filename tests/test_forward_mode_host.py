@@ -63,3 +63,15 @@ def test_the_backward_ops():
         dual = fwAD.make_dual(q, torch.empty_like(q))
         with pytest.raises(NotImplementedError, match="forward AD"):
             OPS.qk_norm_rope_bwd(dual, q, q, q, None, None, None, None, None, 1e-6, False)
+
+
+def test_sdpa():
+    q = meta(2, 3, 9, 64)
+    refuses_a_tangent_of_each(nb.sdpa, (q, q, q), range(3))
+    refuses_a_tangent_of_each(lambda *a: OPS.sdpa_fwd(*a, 0.125), (q, q, q), range(3))
+
+
+def test_sdpa_varlen():
+    q, cu = meta(9, 2, 64), meta(3, dtype=torch.int32)
+    refuses_a_tangent_of_each(lambda *a: nb.sdpa_varlen(*a, cu, cu, 5, 5), (q, q, q), range(3))
+    refuses_a_tangent_of_each(lambda *a: OPS.sdpa_varlen_fwd(*a, cu, cu, 5, 5, 0.125), (q, q, q), range(3))
