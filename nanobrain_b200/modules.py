@@ -109,6 +109,15 @@ class Attention(nn.Module):
         self.k_norm = nn.Parameter(torch.ones(self.head_dim)) if qk_norm else None
         self.register_buffer("rope_freqs", None if rope_grid is None else axial_frequencies(rope_grid), persistent=False)
 
+    def _apply(self, fn: Callable, recurse: bool = True) -> "Attention":
+        # The frequencies move with the module, but keep their type where it is converted: bfloat16 would leave 8 of
+        # their 24 bits, and the operator takes float32.
+        freqs = self.rope_freqs
+        super()._apply(fn, recurse)
+        if freqs is not None and self.rope_freqs.dtype != freqs.dtype:
+            self.rope_freqs = freqs.to(self.rope_freqs.device)
+        return self
+
     def extra_repr(self) -> str:
         return f"num_heads={self.num_heads}, causal={self.causal}"
 
