@@ -40,7 +40,7 @@ typedef struct nb_qk_side {
 
 typedef struct nb_qk_norm_rope_args {
   nb_qk_side q, k;
-  int32_t batch;           /* packed tokens are one sequence */
+  int32_t batch;           /* packed tokens are one sequence; 0: there is nothing to do but zeros in d_weight */
   int32_t axes;            /* position coordinates per token; 0: no rotation */
   int32_t position_type;   /* enum nb_position_type */
   int32_t interleaved;

@@ -402,7 +402,7 @@ int make_side(const nb_qk_side& in, const nb_qk_norm_rope_args& a, bool bwd, Sid
   if (in.heads <= 0 || in.tokens < 0 || in.heads > 65535) return NB_ATTN_ERR_SHAPE;
   if (int64_t(in.tokens) * a.batch > INT32_MAX) return NB_ATTN_ERR_SHAPE;
   if (bwd && in.d_weight == nullptr) return NB_ATTN_ERR_NULL;
-  if (in.tokens > 0) {  // (a side without tokens has no addresses)
+  if (in.tokens > 0 && a.batch > 0) {  // (a side without tokens has no addresses)
     if (int rc = check_tensor(in.x)) return rc;
     if (int rc = check_tensor(in.y)) return rc;
     if (bwd)
@@ -425,7 +425,7 @@ int make_side(const nb_qk_side& in, const nb_qk_norm_rope_args& a, bool bwd, Sid
 
 int make_params(const nb_qk_norm_rope_args* a, bool bwd, Params* p) {
   if (a == nullptr) return NB_ATTN_ERR_NULL;
-  if (a->batch <= 0 || a->axes < 0 || a->axes > NB_ROPE_MAX_AXES || a->position_type < 0 || a->position_type > 2)
+  if (a->batch < 0 || a->axes < 0 || a->axes > NB_ROPE_MAX_AXES || a->position_type < 0 || a->position_type > 2)
     return NB_ATTN_ERR_SHAPE;
   if (a->axes > 0 && a->freqs == nullptr) return NB_ATTN_ERR_NULL;
   *p = Params{};
