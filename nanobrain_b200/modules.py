@@ -143,7 +143,7 @@ class Attention(nn.Module):
         context_coord: Optional[Tensor] = None,
     ) -> Tensor:
         """``coord``: the tokens' grid coordinates, ``[B, N, axes]`` or packed ``[T, axes]``, where the module rotates;
-        ``context_coord``: those of ``context``."""
+        ``context_coord``: those of ``context``. A module that does not rotate does not look at them."""
         src = x if context is None else context
         if context is not None and context_coord is None and self.rope_freqs is not None:
             raise ValueError("context_coord is required with context: its tokens have coordinates of their own")
@@ -255,7 +255,8 @@ class Block(nn.Module):
                 max_seqlen: Optional[int] = None, seq_id: Optional[Tensor] = None, coord: Optional[Tensor] = None,
                 context_coord: Optional[Tensor] = None) -> Tensor:
         num_seqs = None if cu_seqlens is None else cu_seqlens.numel() - 1
-        rotation = {} if coord is None else {"coord": coord, "context_coord": context_coord}
+        rotation = {"coord": coord, "context_coord": context_coord}
+        rotation = {name: t for name, t in rotation.items() if t is not None}
         y = self.attn(self.norm1(x), context=context, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, **rotation)
         x = x + self._drop(self.drop_path1, y, seq_id, num_seqs)
         return x + self._drop(self.drop_path2, self.mlp(self.norm2(x)), seq_id, num_seqs)
