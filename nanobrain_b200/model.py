@@ -194,7 +194,8 @@ class ViTMAE3D(nn.Module):
         vis_mask, target_mask = torch.split(mask_patches, [num_visible, num_predict], dim=1)
         vis_coord, target_coord = torch.split(coord, [num_visible, num_predict], dim=1)
         embeds = self.forward_encoder(vis_patches, vis_coord)
-        pred = self.forward_decoder(embeds, target_coord, coord=vis_coord)
+        rotation = {"coord": vis_coord} if self.rope else {}  # (a decoder that someone has replaced may know of no others)
+        pred = self.forward_decoder(embeds, target_coord, **rotation)
         loss = F.mse_loss(pred, target_patches, reduction="none")
         loss = (target_mask * loss).sum() / target_mask.sum()
         if not with_state:
