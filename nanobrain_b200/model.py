@@ -79,6 +79,8 @@ def _init_weights(m: nn.Module) -> None:
 class ViTMAE3D(nn.Module):
     """3D ViT masked autoencoder with the reference's parameters and a packed-token path."""
 
+    rope = False  # (of a model that was pickled before it had the choice)
+
     def __init__(
         self,
         grid_size: Tuple[int, int, int] = (192, 240, 192),

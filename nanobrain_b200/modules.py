@@ -109,6 +109,12 @@ class Attention(nn.Module):
         self.k_norm = nn.Parameter(torch.ones(self.head_dim)) if qk_norm else None
         self.register_buffer("rope_freqs", None if rope_grid is None else axial_frequencies(rope_grid), persistent=False)
 
+    def __setstate__(self, state: dict) -> None:
+        super().__setstate__(state)
+        for name in ("q_norm", "k_norm"):  # a module that was pickled before it had them
+            self._parameters.setdefault(name, None)
+        self._buffers.setdefault("rope_freqs", None)
+
     def _apply(self, fn: Callable, recurse: bool = True) -> "Attention":
         # The frequencies move with the module, but keep their type where it is converted: bfloat16 would leave 8 of
         # their 24 bits, and the operator takes float32.
