@@ -105,8 +105,8 @@ class Attention(nn.Module):
         self.k = nn.Linear(kv_in, dim, bias=qkv_bias)
         self.v = nn.Linear(kv_in, dim, bias=qkv_bias)
         self.proj = nn.Linear(dim, dim, bias=proj_bias)
-        self.q_norm = nn.Parameter(torch.ones(self.head_dim)) if qk_norm else None
-        self.k_norm = nn.Parameter(torch.ones(self.head_dim)) if qk_norm else None
+        self.register_parameter("q_norm", nn.Parameter(torch.ones(self.head_dim)) if qk_norm else None)
+        self.register_parameter("k_norm", nn.Parameter(torch.ones(self.head_dim)) if qk_norm else None)
         self.register_buffer("rope_freqs", None if rope_grid is None else axial_frequencies(rope_grid), persistent=False)
 
     def __setstate__(self, state: dict) -> None:

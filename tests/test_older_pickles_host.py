@@ -15,7 +15,9 @@ def as_saved_before(model):
     model = copy.deepcopy(model)
     for m in model.modules():
         if isinstance(m, modules.Attention):
-            del m._parameters["q_norm"], m._parameters["k_norm"], m._buffers["rope_freqs"]
+            for name in ("q_norm", "k_norm", "rope_freqs"):
+                for place in (vars(m), m._parameters, m._buffers):
+                    place.pop(name, None)
             m._non_persistent_buffers_set.discard("rope_freqs")
         if isinstance(m, M.ViTMAE3D):
             del m.rope
