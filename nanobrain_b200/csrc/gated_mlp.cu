@@ -287,7 +287,7 @@ int launch(void (*kernel)(Arg), dim3 grid, unsigned threads, size_t smem, void* 
 // A GEMM kernel needs its shared memory allowed once per device.
 constexpr int kMaxDevices = 64;
 template <int kCtas, int kKind, int kAct, int kBits, int kProblems>
-int launch_gemm(const GemmParams<kProblems>& g, int sms, void* stream) {
+int launch_gemm(const GemmParams<kProblems>& g, int sms, int32_t* status, void* stream) {
   static std::mutex mutex;
   static bool ready[kMaxDevices];
   auto* kernel = gemm_kernel<kCtas, kKind, kAct, kBits, kProblems>;
@@ -304,12 +304,12 @@ int launch_gemm(const GemmParams<kProblems>& g, int sms, void* stream) {
     }
   }
   const int units = g.deal.n_long + g.deal.n_short, teams = std::min(units, sms / kCtas);
-  return launch_cluster(kernel, kCtas, dim3(unsigned(teams * kCtas)), kGemmThreads, kSmem, stream, g, GemmTail{g.status, {}});
+  return launch_cluster(kernel, kCtas, dim3(unsigned(teams * kCtas)), kGemmThreads, kSmem, stream, g, GemmTail{status, {}});
 }
 template <int kKind, int kAct, int kBits, int kProblems>
-int launch_gemm(const GemmParams<kProblems>& g, int ctas, int sms, void* stream) {
-  return ctas == 2 ? launch_gemm<2, kKind, kAct, kBits, kProblems>(g, sms, stream)
-                   : launch_gemm<1, kKind, kAct, kBits, kProblems>(g, sms, stream);
+int launch_gemm(const GemmParams<kProblems>& g, int ctas, int sms, int32_t* status, void* stream) {
+  return ctas == 2 ? launch_gemm<2, kKind, kAct, kBits, kProblems>(g, sms, status, stream)
+                   : launch_gemm<1, kKind, kAct, kBits, kProblems>(g, sms, status, stream);
 }
 
 int div_up(int64_t a, int64_t b) { return int((a + b - 1) / b); }
@@ -405,18 +405,18 @@ int launch_few(const nb_gated_mlp_fwd_args& a, void* stream) {
 }
 
 template <int kKind, int kAct>
-int launch_bits(const GemmParams<1>& g, int checkpoint, int ctas, int sms, void* stream) {
+int launch_bits(const GemmParams<1>& g, int checkpoint, int ctas, int sms, int32_t* status, void* stream) {
   switch (checkpoint) {
-    case NB_CHECKPOINT_16BIT: return launch_gemm<kKind, kAct, 16, 1>(g, ctas, sms, stream);
-    case NB_CHECKPOINT_8BIT: return launch_gemm<kKind, kAct, 8, 1>(g, ctas, sms, stream);
+    case NB_CHECKPOINT_16BIT: return launch_gemm<kKind, kAct, 16, 1>(g, ctas, sms, status, stream);
+    case NB_CHECKPOINT_8BIT: return launch_gemm<kKind, kAct, 8, 1>(g, ctas, sms, status, stream);
   }
-  if constexpr (kKind == kGemmGate) return launch_gemm<kKind, kAct, 0, 1>(g, ctas, sms, stream);
+  if constexpr (kKind == kGemmGate) return launch_gemm<kKind, kAct, 0, 1>(g, ctas, sms, status, stream);
   return NB_ATTN_ERR_SHAPE;
 }
 template <int kKind>
-int launch_act(const GemmParams<1>& g, const nb_gated_mlp_shape& s, int ctas, int sms, void* stream) {
-  return s.activation == NB_ACT_SILU ? launch_bits<kKind, kActSilu>(g, s.checkpoint, ctas, sms, stream)
-                                     : launch_bits<kKind, kActGelu>(g, s.checkpoint, ctas, sms, stream);
+int launch_act(const GemmParams<1>& g, const nb_gated_mlp_shape& s, int ctas, int sms, int32_t* status, void* stream) {
+  return s.activation == NB_ACT_SILU ? launch_bits<kKind, kActSilu>(g, s.checkpoint, ctas, sms, status, stream)
+                                     : launch_bits<kKind, kActGelu>(g, s.checkpoint, ctas, sms, status, stream);
 }
 
 // The kernels divide unit numbers (below 2^31) by the column tiles: with 2^(k-1) < d <= 2^k, ceil(2^(31+k) / d) is below 2^32
@@ -558,7 +558,6 @@ extern "C" int nb_gated_mlp_fwd(const nb_gated_mlp_fwd_args* args, void* stream)
   g.codes = static_cast<uint8_t*>(args->checkpoint);
   g.groups = div_up(s.hidden, kGroup), g.hidden = s.hidden;
   g.deal.n_short = p.row_tiles * p.col_tiles;
-  g.status = args->status;
 
   GemmParams<1> d{};
   GemmProblem& q = d.p[0];
@@ -570,9 +569,8 @@ extern "C" int nb_gated_mlp_fwd(const nb_gated_mlp_fwd_args* args, void* stream)
   NB_TRY(host_matrix_map(&q.c, args->y.ptr, s.tokens, s.dim, args->y.stride, 32, 64));
   q.bias = static_cast<const bf16*>(args->b_down);
   d.deal.n_short = q.row_tiles * q.col_tiles;
-  d.status = args->status;
-  NB_TRY(launch_act<kGemmGate>(g, s, tg.ctas, sms, stream));
-  return launch_gemm<kGemmPlain, 0, 0, 1>(d, td.ctas, sms, stream);
+  NB_TRY(launch_act<kGemmGate>(g, s, tg.ctas, sms, args->status, stream));
+  return launch_gemm<kGemmPlain, 0, 0, 1>(d, td.ctas, sms, args->status, stream);
 }
 
 extern "C" size_t nb_gated_mlp_bwd_workspace_bytes(const nb_gated_mlp_bwd_args* args) {
@@ -634,12 +632,10 @@ extern "C" int nb_gated_mlp_bwd(const nb_gated_mlp_bwd_args* args, void* stream)
     g.codes = static_cast<uint8_t*>(const_cast<void*>(a.checkpoint));
     g.groups = div_up(s.hidden, kGroup), g.hidden = s.hidden;
     g.deal.n_short = p.row_tiles * p.col_tiles;
-    g.status = a.status;
   }
 
   // dx and the weight gradients, the longer units first.
   GemmParams<kProducts> g{};
-  g.status = a.status;
   SplitParams sums{};
   int n = 0;
   const auto add = [&](int which, const nb_matrix& out) -> int {
@@ -676,7 +672,7 @@ extern "C" int nb_gated_mlp_bwd(const nb_gated_mlp_bwd_args* args, void* stream)
   NB_TRY(add(kDWUp, a.d_w_up));
   NB_TRY(add(kDWDown, a.d_w_down));
   if (dw_first) NB_TRY(add(kDx, a.dx));
-  if (dact) NB_TRY(launch_act<kGemmDact>(act, s, act_tiling.ctas, sms, stream));
+  if (dact) NB_TRY(launch_act<kGemmDact>(act, s, act_tiling.ctas, sms, a.status, stream));
   if (n > 0) {
     int dw_units = 0;
     for (int i = 0; i < kDx; ++i) dw_units += plan.p[i].wanted ? plan.p[i].units() : 0;
@@ -687,7 +683,7 @@ extern "C" int nb_gated_mlp_bwd(const nb_gated_mlp_bwd_args* args, void* stream)
       const double ratio = dw.unit_clocks() / dx.unit_clocks();
       g.deal.extra = std::min(int(dw_first ? ratio : 1.0 / ratio), g.deal.n_short / (teams - rem));
     }
-    NB_TRY((launch_gemm<kGemmPlain, 0, 0, kProducts>(g, plan.ctas, sms, stream)));
+    NB_TRY((launch_gemm<kGemmPlain, 0, 0, kProducts>(g, plan.ctas, sms, a.status, stream)));
   }
   if (sums.n_items > 0) {
     int64_t pieces = 0;

@@ -101,7 +101,6 @@ template <int kProblems>
 struct GemmParams {
   GemmProblem p[kProblems];
   GemmDeal deal;
-  int32_t* status;
   // the gate's and its backward's
   CUtensorMap map_db, map_h;   // backward (p[0].c is that of da, forward of h)
   const __nv_bfloat16* bias_up;
