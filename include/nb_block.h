@@ -21,7 +21,8 @@ extern "C" {
 
 /* ---- queries and keys: RMS norm over each head's 64 values, then rotation by the token's position ----------
  * n = x / sqrt(mean(x^2) + eps) * weight; pair i of a head (values i and i + 32, or 2 i and 2 i + 1 where
- * `interleaved`) is turned by angle sum_a position[a] * freqs[a][i], computed in 64 bits. */
+ * `interleaved`) is turned by angle sum_a position[a] * freqs[a][i], computed in 64 bits. The sum of squares is in
+ * fp32 (values beyond 1e18 overflow it); results are rounded once. */
 #define NB_ROPE_MAX_AXES 4
 
 enum nb_position_type { NB_POSITION_I32 = 0, NB_POSITION_I64 = 1, NB_POSITION_F32 = 2 };
@@ -60,8 +61,12 @@ size_t nb_qk_norm_rope_bwd_workspace_bytes(void);
 enum nb_activation { NB_ACT_SILU = 0, NB_ACT_GELU = 1 /* with erf */ };
 
 /* What the forward keeps of a = x Wg^T + bg and b = x Wu^T + bu for the backward: in 16 bits fp16 values with a power of
- * two per 32 features of a token (2^-12 of the value or of 2^-29 of the group's largest); in 8 bits whole
- * multiples of max |.| / 127 rounded up to bf16, per 32 features of a token. */
+ * two per 32 features of a token (2^-12 of the value or of 2^-29 of the group's largest; a group with a value that is not
+ * finite is kept as plain fp16); in 8 bits whole multiples of max |.| / 127 rounded up to bf16, per 32 features of a token
+ * (zeros where that is below 2^-100; a group with a value that is not finite is NaN as a whole).
+ *
+ * Products are summed in fp32. What a product takes from another is rounded to bf16 first, as the tensor cores want it:
+ * act(a) b in front of Wd, and in the backward the gradients of a and b (those of the biases are summed before that). */
 enum nb_checkpoint { NB_CHECKPOINT_NONE = 0, NB_CHECKPOINT_16BIT = 1, NB_CHECKPOINT_8BIT = 2 };
 
 typedef struct nb_matrix {

@@ -148,7 +148,8 @@ def qk_norm_rope(
     them nothing is turned. ``k_positions``: of the keys, where they are other tokens than the queries. Neither
     positions nor frequencies have a gradient.
 
-    Every token is treated by itself, rows behind the last sequence of a packed buffer too."""
+    Every token is treated by itself, rows behind the last sequence of a packed buffer too. The sum of squares is
+    in float32 (values beyond 1e18 overflow it); the result is rounded once."""
     if _observed(q, k, q_weight, k_weight, positions, k_positions, freqs):
         return qk_norm_rope_fwd(q, k, q_weight, k_weight, positions, k_positions, freqs, float(eps), bool(interleaved))
     native = ops._native or ops._load_native()
@@ -179,7 +180,12 @@ def gated_mlp(
       (6 bytes per token and feature in all);
     * ``"8bit"``: whole multiples of ``max|.| / 127`` (rounded up to bfloat16) per 32 features of a token
       (2.1 bytes per token and feature; the inner activations are computed again from them). The gradients are
-      then those at the rounded ``a`` and ``b``. A group with a value that is not finite is NaN as a whole."""
+      then those at the rounded ``a`` and ``b``. A group whose multiple would be below 2^-100 is zeros, one with a
+      value that is not finite is NaN as a whole.
+
+    Products are summed in float32; the inner activations and, in the backward, the gradients of ``a`` and ``b`` are
+    rounded to bfloat16 between two products, as the results are at the end (errors of 0.0025 against 0.0017 of the
+    result's rounding alone)."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
     if checkpoint not in _CHECKPOINTS:

@@ -13,8 +13,8 @@
 // Large products are made by pairs of CTAs (cta_group::2) on tiles of 256 rows x 256 columns: each CTA loads its 128 rows
 // of A and half of B. What bounds one CTA's 128 x 256 tile is its shared memory's port (128 bytes a clock): a 64-deep
 // step takes 512 clocks of MMAs, but its 48 KB are written once and read once, 768 clocks. A pair's CTA moves 32 KB. Measured
-// on 26253 x 768 x 2048 (one training step): gate 126 us (1.31 PFLOP/s), y 63 (1.31), activation's backward 93 (0.89, 440 MB), dx and
-// the weight gradients 267 (1.86).
+// on 26253 x 768 x 2048 (one training step; boards differ by 5 %): gate 126-130 us (1.27-1.31 PFLOP/s), y 63-64 (1.29-1.31),
+// activation's backward 93-96 (0.86-0.89, 440 MB), dx and the weight gradients, five products, 267-279 (1.48-1.55).
 #pragma once
 
 #include <cuda_fp16.h>

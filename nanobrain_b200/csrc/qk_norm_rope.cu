@@ -10,7 +10,7 @@
 // [32+8j, 32+8j+8), which contain both partners of every pair in either order of pairs, so the rotation needs no
 // exchange and every access is 16 bytes. A lane keeps its eight pairs as first and second partners, two pairs to a
 // packed instruction: with one value per instruction the kernels took 35 (forward) and 72 us (backward) on 26253 tokens of
-// 12 + 12 heads, bound by their instructions; now 31 and 53 (161 and 242 MB: 5.2 and 4.6 TB/s). Sums are in fp32; the one
+// 12 + 12 heads, bound by their instructions; now 33 and 54 (161 and 242 MB: 4.9 and 4.5 TB/s). Sums are in fp32; the one
 // rounding is that of the result to bf16. Angles are products and sums in 64 bits, and whole turns are taken off there: position 2^20 at
 // frequency 1 would keep an error of 0.03 in fp32.
 #include <cuda_bf16.h>
