@@ -604,8 +604,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             wa[4 * c] = x.x, wa[4 * c + 1] = x.y, wa[4 * c + 2] = x.z, wa[4 * c + 3] = x.w;
             wb[4 * c] = y.x, wb[4 * c + 1] = y.y, wb[4 * c + 2] = y.z, wb[4 * c + 3] = y.w;
           }
+          // The block has been read, by every lane, before the copy that refills it may write: without the fence nothing orders
+          // these loads in front of the async proxy's writes, and one in some 25000 calls found the next block's values.
+          fence_proxy_async_smem();
           __syncwarp();
-          request(slot);  // the block has been read
+          request(slot);
           tmem_wait_ld32(r);
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
